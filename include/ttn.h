@@ -40,7 +40,9 @@ typedef enum ttn_status {
   TTN_DEVICE_FAULT_FLAG = 5  /* a kernel raised its device status word */
 } ttn_status;
 
-typedef enum ttn_dtype { TTN_F16 = 0, TTN_F32 = 1 } ttn_dtype;
+/* TTN_BF16 is taken only by the entry points that say so (the language-model
+ * section); the others refuse it with TTN_UNSUPPORTED. */
+typedef enum ttn_dtype { TTN_F16 = 0, TTN_F32 = 1, TTN_BF16 = 2 } ttn_dtype;
 
 typedef enum ttn_binary_op {
   TTN_SUB = 0, /* x - alpha*y */
@@ -388,6 +390,73 @@ ttn_status ttn_select_f16(const ttn_tensor* decoded, int64_t max_det, uint32_t f
  * This entry point has no counterpart in the reference. */
 ttn_status ttn_select_f16_static(const ttn_tensor* decoded, int64_t max_det, uint32_t flags,
                                  float* out, const ttn_select_trace* trace, ttn_stream stream);
+
+/* ------------------------------------------- language models: experts, read-out
+ * Routing to experts, the experts' gated products and the log probabilities of given
+ * tokens: the serving operators of a mixture-of-experts language model.  f16 or bf16
+ * activations and weights (the two score operators take f32 rows too), FP32 and wider
+ * arithmetic.  These entry points have no counterpart in the reference; the nearest
+ * are its row softmax (softmax_host.cpp:51-89), its device-resident top-k
+ * (selection_flow.cpp:429-491) and its convolution with a SiLU epilogue
+ * (conv_flow.cpp:594-646). */
+
+/* Router.  logits: f16, bf16 or f32 [rows, experts], any strides; 1..1024 experts.
+ * Scores s = softmax over the row, or sigmoid with TTN_ROUTE_SIGMOID; rank = s + bias
+ * (f32 [experts] or NULL).  groups > 1 splits the experts into that many equal runs,
+ * ranks each by its best rank (group_top 1) or the sum of its two best (2) and keeps
+ * the top_groups best.  The top_k (1..16) experts by rank are chosen from those;
+ * experts [rows, top_k] int32 receives them in falling rank, equal ranks (of experts
+ * and of groups) in index order, and weights [rows, top_k] f32 their s (without the bias) times `scale`,
+ * with TTN_ROUTE_RENORMALIZE divided by the sum of the chosen s first (0 where that is
+ * 0).  The order is that of the exact ranks: fp32 scores too close to tell apart are
+ * ranked again in 64 bits, and without a bias the logits themselves are compared.
+ * A logit of -inf masks its expert: it is never chosen, and choices for which no
+ * expert is left get id -1 and weight 0.  A NaN ranks first; in a softmax row a NaN or
+ * +inf makes every score NaN.  Both outputs contiguous. */
+#define TTN_ROUTE_SIGMOID 1u
+#define TTN_ROUTE_RENORMALIZE 2u
+ttn_status ttn_route_experts(const ttn_tensor* logits, const float* bias, int64_t top_k, int64_t groups,
+                             int64_t top_groups, int32_t group_top, uint32_t flags, float scale,
+                             float* weights, int32_t* experts, ttn_stream stream);
+
+/* Log probabilities of given tokens.  logits: f16, bf16 or f32 [rows, vocabulary] with a
+ * unit last stride (any row stride), vocabulary 1..2^20.  With p = softmax(scale * row):
+ *   logprobs [rows]      log p(tokens[row]); 0 where tokens[row] is outside the
+ *                        vocabulary (a row without a given token), NULL with NULL tokens
+ *   entropy [rows]       -sum p log p
+ *   top_logprobs, top_tokens [rows, top]   the top (0..32) largest in falling order,
+ *                        equal logits in index order
+ * all f32 (tokens int64, top_tokens int32), contiguous.  Logits of -inf are masked:
+ * p = 0, log p = -inf, never among the top (left-over places: -inf and token -1); a row
+ * with nothing left has log p = -inf and entropy 0.  A NaN or +inf in a row makes its
+ * logprobs (of a given token), entropy and top_logprobs NaN; top_tokens then still come
+ * in order, NaN first.  scale: finite, > 0.  Any of the outputs but top_* may be NULL. */
+ttn_status ttn_token_logprobs(const ttn_tensor* logits, const int64_t* tokens, float scale, int64_t top,
+                              float* logprobs, float* entropy, float* top_logprobs, int32_t* top_tokens,
+                              ttn_stream stream);
+
+/* Gated products of the chosen experts (no host round trip: the rows of each expert are
+ * found on the device):
+ *   out[t] = sum over j of weights[t][j] * down[e] (silu(gate[e] x[t]) * (up[e] x[t])),
+ *   e = experts[t][j]; the sum in the order of j, silu(v) = v / (1 + exp(-v)).
+ * x: [tokens, hidden], row t at x + t*x_row_stride; experts int32 and weights f32
+ * [tokens, top_k] (ttn_route_experts' outputs); gate_up: [num_experts, 2*inner, hidden]
+ * (an expert's gate rows, then its up rows); down: [num_experts, hidden, inner]; out:
+ * [tokens, hidden], row t at out + t*out_row_stride, must not overlap the inputs.
+ * dtype TTN_F16 or TTN_BF16 for x, gate_up, down and out.  Ids outside 0..num_experts-1
+ * (-1: no choice; another rank's experts) add nothing; a token without any other id
+ * gets zeros.  Products accumulate in FP32; the gated activations are rounded to dtype
+ * between the two products where the tensor cores take them, nothing else is rounded
+ * before out.  hidden % 8 == 0, inner % 16 == 0, 16-byte aligned bases, row strides
+ * multiples of 8; tokens * top_k < 2^31 / 256, top_k 1..32.  workspace: at least
+ * ttn_expert_mlp_workspace_size bytes (0 for malformed sizes), 256-byte aligned, used by
+ * one call at a time. */
+size_t ttn_expert_mlp_workspace_size(int64_t tokens, int64_t hidden, int64_t inner, int64_t num_experts,
+                                     int64_t top_k);
+ttn_status ttn_expert_mlp(int dtype, const void* x, int64_t x_row_stride, int64_t tokens, int64_t hidden,
+                          const int32_t* experts, const float* weights, int64_t top_k, const void* gate_up,
+                          const void* down, int64_t num_experts, int64_t inner, void* out,
+                          int64_t out_row_stride, void* workspace, size_t workspace_bytes, ttn_stream stream);
 
 #ifdef __cplusplus
 }

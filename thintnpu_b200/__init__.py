@@ -10,8 +10,8 @@ from . import _lib
 from . import ops  # noqa: E402
 from .ops import (add, add_silu, attention, bias_silu_residual, cat, contiguous, conv2d, conv2d_pack_weights,
                   copy_, depthwise, depthwise_pack_weights, detection_select,  # noqa: E402,F401
-                  dfl_decode, div, maxpool2d, maxpool_blocked, mul, pack, sigmoid, silu, silu_,
-                  softmax, sppf, sub, unpack, upsample_blocked, upsample_nearest2d)
+                  dfl_decode, div, expert_mlp, maxpool2d, maxpool_blocked, mul, pack, route_experts,
+                  sigmoid, silu, silu_, softmax, sppf, sub, token_logprobs, unpack, upsample_blocked, upsample_nearest2d)
 
 __version__ = "0.1.0"
 

@@ -11,12 +11,13 @@ import os
 from pathlib import Path
 
 MAX_DIMS = 8
-F16, F32 = 0, 1
+F16, F32, BF16 = 0, 1, 2
 SUB, MUL, DIV, ADD = 0, 1, 2, 3
 NCHW, NC1HWC0 = 0, 1
 SELECT_AGNOSTIC, SELECT_NAN_LAST, SELECT_SIGMOID = 1, 2, 4
 ATTENTION_PRESCALE = 1
 CONV_SILU, CONV_NCHW = 1, 2
+ROUTE_SIGMOID, ROUTE_RENORMALIZE = 1, 2
 
 STATUS = {0: "TTN_OK", 1: "TTN_INVALID_ARG", 2: "TTN_UNSUPPORTED", 3: "TTN_CUDA_ERROR",
           4: "TTN_TIMEOUT", 5: "TTN_DEVICE_FAULT_FLAG"}
@@ -36,6 +37,7 @@ EXPORTS = (
     "ttn_conv2d_nc1hwc0_f16", "ttn_conv2d_residual_nc1hwc0_f16", "ttn_conv2d_pack_weights_f16",
     "ttn_conv2d_fault_f16", "ttn_conv2d_test_withhold_copies", "ttn_depthwise_nc1hwc0_f16",
     "ttn_select_workspace_size", "ttn_select_f16", "ttn_select_f16_static",
+    "ttn_route_experts", "ttn_token_logprobs", "ttn_expert_mlp_workspace_size", "ttn_expert_mlp",
 )
 
 
@@ -123,6 +125,12 @@ _SIGNATURES = {
                                       ctypes.POINTER(SelectTrace), _P]),
     "ttn_select_f16_static": (ctypes.c_int, [_TP, _I64, ctypes.c_uint32, _P,
                                              ctypes.POINTER(SelectTrace), _P]),
+    "ttn_route_experts": (ctypes.c_int, [_TP, _P, _I64, _I64, _I64, _I32, ctypes.c_uint32, ctypes.c_float, _P, _P,
+                                         _P]),
+    "ttn_token_logprobs": (ctypes.c_int, [_TP, _P, ctypes.c_float, _I64, _P, _P, _P, _P, _P]),
+    "ttn_expert_mlp_workspace_size": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, _I64]),
+    "ttn_expert_mlp": (ctypes.c_int, [ctypes.c_int, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _P, _I64,
+                                      _P, ctypes.c_size_t, _P]),
 }
 
 _lib = None

@@ -7,7 +7,8 @@ flow_ops.cpp:255-266, selection_flow.cpp:503-514, conv_blocked.cpp:199-206):
 * ``thin_native_flow::{maxpool, upsample, detection_select, detection_select_trace}``,
   the convolutions ``conv`` (conv_flow.cpp:630-646), ``depthwise``
   (depthwise_flow.cpp:225-233) and ``pack_input``, plus the fused ops of this
-  build: ``silu_``, ``sppf``, ``softmax``, ``dfl_decode``, ``bias_silu_residual``
+  build: ``silu_``, ``sppf``, ``softmax``, ``dfl_decode``, ``bias_silu_residual``, and the
+  language-model operators ``route_experts``, ``expert_mlp``, ``token_logprobs``
 * ``thin_blocked::{pack, unpack, conv}`` (conv_blocked.cpp:198-210)
 
 Each op has a CUDA kernel (libttn through ``thintnpu_b200.ops``), a Meta kernel
@@ -209,6 +210,40 @@ def _blocked_conv_meta(x, packed, bias, co, kernel, stride, fp32_output=False, f
     return _conv_meta(x, packed, bias, co, kernel, stride)
 
 
+def _route_cuda(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, group_top=1,
+                renormalize=False, scale=1.0):
+    return ops.route_experts(logits, top_k, score=score, bias=bias, groups=groups, top_groups=top_groups,
+                             group_top=group_top, renormalize=renormalize, scale=scale)
+
+
+def _route_meta(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, group_top=1,
+                renormalize=False, scale=1.0):
+    _require(logits.dim() == 2 and 1 <= top_k <= logits.size(1), "route_experts: top_k must be in [1, experts]")
+    shape = (logits.size(0), top_k)
+    return logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int32)
+
+
+def _mlp_cuda(x, experts, weights, gate_up, down):
+    return ops.expert_mlp(x, experts, weights, gate_up, down)
+
+
+def _mlp_meta(x, experts, weights, gate_up, down):
+    _require(x.dim() == 2 and gate_up.dim() == 3 and gate_up.size(2) == x.size(1),
+             "expert_mlp: gate_up must be [experts, 2*inner, hidden]")
+    return x.new_empty(x.shape)
+
+
+def _logprobs_cuda(logits, tokens, top=0, scale=1.0):
+    return ops.token_logprobs(logits, tokens, top=top, scale=scale)
+
+
+def _logprobs_meta(logits, tokens, top=0, scale=1.0):
+    _require(logits.dim() == 2 and 0 <= top <= logits.size(1), "token_logprobs: top must be in [0, vocabulary]")
+    rows = logits.size(0)
+    new = lambda shape, dtype=torch.float32: logits.new_empty(shape, dtype=dtype)
+    return new((rows,)), new((rows,)), new((rows, top)), new((rows, top), torch.int32)
+
+
 # --------------------------------------------------------------- thin_blocked
 
 def _pack_cuda(x):
@@ -261,6 +296,14 @@ def register() -> None:
     _register(nf, "depthwise(Tensor x, Tensor packed, Tensor? bias, int kernel, int stride, bool fused=True) -> Tensor",
               _depthwise_cuda, _depthwise_meta)
     _register(nf, "pack_input(Tensor x) -> Tensor", _pack_cuda, _pack_meta)
+    _register(nf, "route_experts(Tensor logits, int top_k, str score='softmax', Tensor? bias=None, int groups=1, "
+                  "int? top_groups=None, int group_top=1, bool renormalize=False, float scale=1.0) -> "
+                  "(Tensor weights, Tensor experts)", _route_cuda, _route_meta)
+    _register(nf, "expert_mlp(Tensor x, Tensor experts, Tensor weights, Tensor gate_up, Tensor down) -> Tensor",
+              _mlp_cuda, _mlp_meta)
+    _register(nf, "token_logprobs(Tensor logits, Tensor tokens, int top=0, float scale=1.0) -> "
+                  "(Tensor logprobs, Tensor entropy, Tensor top_logprobs, Tensor top_tokens)",
+              _logprobs_cuda, _logprobs_meta)
     bl = _lib("thin_blocked")
     _register(bl, "pack(Tensor x) -> Tensor", _pack_cuda, _pack_meta)
     _register(bl, "unpack(Tensor x) -> Tensor", _unpack_cuda, _unpack_meta)

@@ -603,3 +603,156 @@ def detection_select(decoded: torch.Tensor, max_det: int, agnostic: bool = False
     if not trace:
         return output
     return [output] + [tensors[name] for name in TRACE_NAMES[1:]]
+
+
+# ------------------------------------------------------------------ language models
+
+_ROW_DTYPES = {torch.float16: _lib.F16, torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
+def _call_on(device: torch.device, function: str, *args) -> None:
+    """``call`` with the current stream of the tensors' device, which becomes the current
+    device for the launch where it is another one."""
+    if device.index == torch.cuda.current_device():
+        call(function, *args, torch.cuda.current_stream().cuda_stream)
+        return
+    with torch.cuda.device(device):
+        call(function, *args, torch.cuda.current_stream().cuda_stream)
+
+
+def _score_rows(x: torch.Tensor, what: str) -> TtnTensor:
+    """Descriptor of a [rows, columns] view of f16, bf16 or f32 scores."""
+    _cuda(x, what)
+    _require(x.dim() == 2, f"{what}: logits must be [rows, columns]")
+    dtype = _ROW_DTYPES.get(x.dtype)
+    _require(dtype is not None, f"{what}: unsupported dtype {x.dtype}: float16/bfloat16/float32 only")
+    d = TtnTensor(x.data_ptr(), 2, dtype)
+    d.sizes[0], d.sizes[1] = x.shape
+    d.strides[0], d.strides[1] = x.stride()
+    return d
+
+
+def _like_output(t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device, what: str) -> None:
+    _require(isinstance(t, torch.Tensor) and tuple(t.shape) == shape and t.dtype == dtype and t.device == device
+             and t.is_contiguous(), f"{what} must be contiguous {dtype} {list(shape)} on {device}")
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
+                  groups: int = 1, top_groups: Optional[int] = None, group_top: int = 1, renormalize: bool = False,
+                  scale: float = 1.0, out: Optional[tuple] = None):
+    """Routing to experts: ``(weights float32 [rows, top_k], experts int32 [rows, top_k])``.
+
+    logits: [rows, experts] f16, bf16 or f32 (any strides, at most 1024 experts).  Scores
+    are the row's ``softmax`` or ``sigmoid``; experts are ranked by score + ``bias``
+    (float32 [experts]), with ``groups`` > 1 only inside the ``top_groups`` groups whose
+    best rank (``group_top`` 1) or sum of two best ranks (2) is largest.  The ``top_k``
+    (at most 16) best come in falling rank, ties to the lower index, ranked as their
+    exact values are; their weights are the scores (without the bias), divided by their
+    sum with ``renormalize``, times ``scale``.  Logits of -inf are never chosen: places
+    for which no expert is left hold id -1 and weight 0.  ``out`` is a (weights, experts)
+    pair to fill."""
+    what = "route_experts"
+    d = _score_rows(logits, what)
+    _require(score in ("softmax", "sigmoid"), f"{what}: score must be 'softmax' or 'sigmoid'")
+    rows, experts = logits.shape
+    device = logits.device
+    bias_ptr = None
+    if bias is not None:
+        _cuda(bias, what)
+        _like_output(bias, (experts,), torch.float32, device, f"{what}: bias")
+        bias_ptr = bias.data_ptr()
+    top_k = int(top_k)
+    _require(1 <= top_k <= experts, f"{what}: top_k must be in [1, experts]")
+    if out is None:
+        weights = torch.empty((rows, top_k), dtype=torch.float32, device=device)
+        ids = torch.empty((rows, top_k), dtype=torch.int32, device=device)
+    else:
+        weights, ids = out
+        _like_output(weights, (rows, top_k), torch.float32, device, f"{what}: out weights")
+        _like_output(ids, (rows, top_k), torch.int32, device, f"{what}: out experts")
+    flags = (_lib.ROUTE_SIGMOID if score == "sigmoid" else 0) | (_lib.ROUTE_RENORMALIZE if renormalize else 0)
+    _call_on(device, "ttn_route_experts", _ref(d), bias_ptr, top_k, groups,
+             groups if top_groups is None else top_groups, group_top, flags, scale, weights.data_ptr(),
+             ids.data_ptr())
+    return weights, ids
+
+
+def expert_mlp_workspace_size(tokens: int, hidden: int, inner: int, num_experts: int, top_k: int) -> int:
+    """Bytes of scratch ``expert_mlp`` needs at these sizes."""
+    return int(_lib.lib().ttn_expert_mlp_workspace_size(tokens, hidden, inner, num_experts, top_k))
+
+
+def expert_mlp(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, gate_up: torch.Tensor,
+               down: torch.Tensor, *, out: Optional[torch.Tensor] = None,
+               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gated products of the chosen experts: ``out[t] = sum_j weights[t, j] * down[e] @
+    (silu(gate[e] @ x[t]) * (up[e] @ x[t]))`` with ``e = experts[t, j]``.
+
+    x: [tokens, hidden] f16 or bf16 (rows of unit stride, 16-byte aligned); experts int32
+    and weights float32 [tokens, top_k], as ``route_experts`` returns them; gate_up:
+    [E, 2*inner, hidden] (gate rows, then up rows) and down: [E, hidden, inner],
+    contiguous, of x's dtype; hidden a multiple of 8, inner of 16.  Ids outside 0..E-1
+    add nothing (-1: no choice; experts of another rank).  Sums are FP32; the gated
+    activations are rounded to x's dtype between the two products (with few pairs they
+    stay FP32), so they have to lie in its range.  ``workspace``: at least
+    ``expert_mlp_workspace_size`` bytes of uint8, 256-byte aligned, for one call at a time."""
+    what = "expert_mlp"
+    for t in (x, experts, weights, gate_up, down):
+        _cuda(t, what)
+    device, dtype = x.device, x.dtype
+    _require(dtype == torch.float16 or dtype == torch.bfloat16, f"{what} supports float16/bfloat16")
+    _require(x.dim() == 2 and (x.stride(1) == 1 or x.size(1) == 1), f"{what}: x must be [tokens, hidden] with unit-stride rows")
+    tokens, hidden = x.shape
+    _require(gate_up.dim() == 3 and gate_up.size(1) % 2 == 0 and gate_up.size(2) == hidden,
+             f"{what}: gate_up must be [experts, 2*inner, hidden]")
+    num, inner = gate_up.size(0), gate_up.size(1) // 2
+    _require(gate_up.dtype == dtype and gate_up.device == device and gate_up.is_contiguous(),
+             f"{what}: gate_up must be contiguous, of x's dtype and device")
+    _like_output(down, (num, hidden, inner), dtype, device, f"{what}: down")
+    _require(experts.dim() == 2 and experts.size(0) == tokens, f"{what}: experts must be [tokens, top_k]")
+    top_k = experts.size(1)
+    _like_output(experts, (tokens, top_k), torch.int32, device, f"{what}: experts")
+    _like_output(weights, (tokens, top_k), torch.float32, device, f"{what}: weights")
+    if out is None:
+        out = torch.empty((tokens, hidden), dtype=dtype, device=device)
+    else:
+        _require(out.shape == x.shape and out.dtype == dtype and out.device == device
+                 and (out.stride(1) == 1 or hidden == 1), f"{what}: out must match x, with unit-stride rows")
+    need = expert_mlp_workspace_size(tokens, hidden, inner, num, top_k)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    else:
+        _require(workspace.dtype == torch.uint8 and workspace.device == device and workspace.is_contiguous(),
+                 f"{what}: workspace must be contiguous uint8 on x's device")
+    _call_on(device, "ttn_expert_mlp", _ROW_DTYPES[dtype], x.data_ptr(), x.stride(0), tokens, hidden,
+             experts.data_ptr(), weights.data_ptr(), top_k, gate_up.data_ptr(), down.data_ptr(), num, inner,
+             out.data_ptr(), out.stride(0), workspace.data_ptr(), workspace.numel())
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, scale: float = 1.0):
+    """Log probabilities of given tokens under ``softmax(scale * logits)``:
+    ``(logprobs [rows], entropy [rows], top_logprobs [rows, top], top_tokens [rows, top])``,
+    float32 and (the last) int32.
+
+    logits: [rows, vocabulary] f16, bf16 or f32, unit last stride, any row stride, at most
+    2^20 columns; tokens: int64 [rows].  A token outside the vocabulary marks a row
+    without a given token: its log probability is 0.  The ``top`` (at most 32) largest
+    come in falling order, ties to the lower index.  Logits of -inf are masked: never
+    among the top (left-over places hold -inf and token -1), log probability -inf; a row
+    with nothing left has entropy 0.  A NaN or +inf in a row makes its log probabilities
+    and entropy NaN."""
+    what = "token_logprobs"
+    d = _score_rows(logits, what)
+    rows, device = logits.size(0), logits.device
+    _cuda(tokens, what)
+    _like_output(tokens, (rows,), torch.int64, device, f"{what}: tokens")
+    top = int(top)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+    entropy = torch.empty(rows, dtype=torch.float32, device=device)
+    _require(0 <= top <= logits.size(1), f"{what}: top must be in [0, vocabulary]")
+    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
+    top_tokens = torch.empty((rows, top), dtype=torch.int32, device=device)
+    _call_on(device, "ttn_token_logprobs", _ref(d), tokens.data_ptr(), scale, top, logprobs.data_ptr(),
+             entropy.data_ptr(), top_logprobs.data_ptr() if top else None, top_tokens.data_ptr() if top else None)
+    return logprobs, entropy, top_logprobs, top_tokens
