@@ -458,6 +458,11 @@ ttn_status ttn_expert_mlp(int dtype, const void* x, int64_t x_row_stride, int64_
                           const void* down, int64_t num_experts, int64_t inner, void* out,
                           int64_t out_row_stride, void* workspace, size_t workspace_bytes, ttn_stream stream);
 
+/* Reads and clears the fault word of the experts' products: nonzero when a launch gave
+ * up waiting (1 = an operand copy, 2 = a free ring stage, 4 = an accumulator); its
+ * output is then incomplete.  Synchronous. */
+ttn_status ttn_expert_mlp_fault(uint32_t* fault);
+
 #ifdef __cplusplus
 }
 #endif

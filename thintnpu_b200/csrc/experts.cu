@@ -3,10 +3,34 @@
 //
 // Few pairs (token, choice): the experts' weights are read once for each pair by
 // ordinary warps, two launches in all (expert_rows_gate_up, expert_rows_down).
+//
+// More pairs: the tensor cores, four launches.
+//  * expert_plan sorts the pairs by expert (stable): offsets[E + 1], order[pairs].
+//  * expert_products<gate-up> and <down>: grouped matrix products on pairs of CTAs
+//    (tcgen05, cta_group::2), persistent and warp-specialised.  The weights are the M
+//    operand (128 rows a CTA) and an expert's rows the N operand (32 to 256 in steps of
+//    32), so an expert with few rows costs few columns, and a batch of single tokens
+//    streams each expert's weights once through tiles 32 columns wide.
+//    - The rows of x are gathered by TMA (tile::gather4) through `order`: no sorted copy.
+//    - A CTA's 128 weight rows of the first product are 4 x (16 gate rows, 16 up rows),
+//      one TMA box of a five-dimensional map, so that the gate and up values of a feature
+//      sit in lanes l and l + 16 of one warp: one shuffle a value pair, then
+//      silu(gate) * up, rounded to the operands' type for the second product.
+//    - The second product's values, one pair's share of an output, are kept in 16 bits:
+//      integers times an FP32 scale for each 32 features of a pair (a warp's lanes), exact
+//      to 2^-16 of the largest of the 32, where a rounding to bf16 would be off by 2^-9.
+//  * expert_combine adds a token's shares in the order of its choices.
+// Every wait is bounded (200 ms); a role that gives up records why in a device word
+// (ttn_expert_mlp_fault) and the pair frees its TMEM and returns.
+#include <type_traits>
+
 #include "rows.cuh"
+#include "tcgen05.cuh"
 
 namespace ttn {
 namespace {
+
+using namespace tc;
 
 constexpr uint32_t kAll = 0xffffffffu;
 constexpr int kMaxExperts = 1024;
@@ -127,23 +151,459 @@ __global__ void __launch_bounds__(kDownWarps * 32) expert_rows_down(ExpertArgs a
   }
 }
 
+// ------------------------------------------------------------ tensor cores
+
+__device__ uint32_t g_expert_fault;
+
+// offsets[e]: pairs of experts below e; order: the pairs, by expert, then by number.  One
+// block an expert, each reading all ids (they are few and in L2): no block waits for another.
+constexpr int kPlanThreads = 512;
+constexpr int kPlanWarps = kPlanThreads / 32;
+__global__ void __launch_bounds__(kPlanThreads) expert_plan(const int32_t* __restrict__ ids, int pairs, int experts,
+                                                            int32_t* __restrict__ offsets, int32_t* __restrict__ order) {
+  __shared__ int below[kPlanWarps], mine[kPlanWarps];
+  pdl_trigger();
+  pdl_wait();
+  const int e = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunk = (pairs + kPlanWarps * 32 - 1) / (kPlanWarps * 32) * 32;
+  const int64_t first = (int64_t)warp * chunk;
+  const int64_t last = first + chunk < pairs ? first + chunk : pairs;
+  int less = 0, equal = 0;
+  for (int64_t i = first + lane; i < last; i += 32) {
+    const int id = ids[i];
+    less += (unsigned)id < (unsigned)e;
+    equal += id == e;
+  }
+  less = __reduce_add_sync(kAll, less);
+  equal = __reduce_add_sync(kAll, equal);
+  if (lane == 0) below[warp] = less, mine[warp] = equal;
+  __syncthreads();
+  int at = 0, total = 0;
+  for (int w = 0; w < kPlanWarps; ++w) {
+    at += below[w] + (w < warp ? mine[w] : 0);
+    total += below[w] + mine[w];
+  }
+  if (threadIdx.x == 0) {
+    offsets[e] = at;  // warp 0: nothing of this expert before it
+    if (e == experts - 1) offsets[experts] = total;
+  }
+  if (!equal) return;
+  for (int64_t i0 = first; i0 < last; i0 += 32) {
+    const int64_t i = i0 + lane;
+    const bool in = i < last && ids[i] == e;
+    const uint32_t vote = __ballot_sync(kAll, in);
+    if (in) order[at + __popc(vote & ((1u << lane) - 1))] = (int)i;
+    at += __popc(vote);
+  }
+}
+
+constexpr int kTileN = 256;      // rows of an expert in a tile, at most
+constexpr int kStepK = 64;       // reduction elements of a ring stage: 128 bytes, the swizzle's width
+constexpr int kStages = 6;
+constexpr uint32_t kABytes = 128 * kStepK * 2, kBBytes = kTileN / 2 * kStepK * 2;
+constexpr uint32_t kStageBytes = kABytes + kBBytes;
+constexpr int kEpiWarps = 8;
+constexpr int kProductThreads = 64 + 32 * kEpiWarps;
+constexpr uint32_t kStagingBytes = 32 * 64;  // one epilogue warp: 32 rows x 64 bytes
+constexpr int kShareBlock = 32;              // features that share a scale
+
+struct ProductArgs {
+  const int32_t *offsets, *order;
+  uint16_t* h;      // gate-up: [pairs, sorted][inner]
+  int16_t* share;   // down: [pair][hidden], integers (or bf16 where the scale is negative)
+  float* scale;     // down: [pair][blocks]
+  int experts, top_k, rows, steps, m_tiles, blocks;  // rows: weight rows of the product (inner or hidden)
+  int bf16;
+};
+struct ProductMaps {
+  CUtensorMap a, b;
+};
+__host__ __device__ constexpr uint32_t product_smem(int experts) {
+  return 1024 + kStages * kStageBytes + kEpiWarps * kStagingBytes + 2 * 4 * (uint32_t)(experts + 1);
+}
+
+// Tile t of the list: experts in order, of an expert its runs of rows, of a run its weight rows.
+struct TileList {
+  const int32_t *offsets, *tiles;  // shared memory: offsets[E + 1], runs before each expert [E + 1]
+  int m_tiles, e;
+  // -> expert, first weight-row tile, first sorted row, rows; t must not fall from call to call
+  __device__ __forceinline__ void at(int t, int& m, int& row, int& count) {
+    const int run = t / m_tiles;
+    m = t - run * m_tiles;
+    while (tiles[e + 1] <= run) ++e;
+    const int all = offsets[e + 1] - offsets[e], runs = tiles[e + 1] - tiles[e];
+    const int n = ((all + runs - 1) / runs + 31) & ~31;  // equal runs, in steps of 32 rows
+    const int i = run - tiles[e];
+    row = offsets[e] + i * n;
+    count = min(n, all - i * n);
+  }
+};
+
+template <typename T, bool kGateUp>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
+    expert_products(ProductArgs a, const __grid_constant__ ProductMaps maps) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 4];  // full[s], empty[s], acc_full[2], acc_empty[2]
+  __shared__ uint32_t tmem_slot;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
+  const uint32_t smem0 = ((uint32_t)__cvta_generic_to_shared(smem) + 1023u) & ~1023u;
+  unsigned char* generic0 = smem + (smem0 - (uint32_t)__cvta_generic_to_shared(smem));
+  unsigned char* staging = generic0 + kStages * kStageBytes;
+  int32_t* offsets = reinterpret_cast<int32_t*>(staging + kEpiWarps * kStagingBytes);
+  int32_t* tiles = offsets + a.experts + 1;
+  const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(&bars[0]);
+  auto full_bar = [&](int s) { return bar0 + 8 * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8 * (kStages + s); };
+  auto acc_full = [&](int i) { return bar0 + 8 * (2 * kStages + i); };
+  auto acc_empty = [&](int i) { return bar0 + 8 * (2 * kStages + 2 + i); };
+
+  pdl_trigger();
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full_bar(s), 1);   // the leader's: its producer, and both CTAs' bytes
+      mbar_init(empty_bar(s), 1);  // the products' commit
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full(i), 1);
+      mbar_init(acc_empty(i), 2 * kEpiWarps);  // the leader's: both CTAs' epilogue warps
+    }
+    mbar_init_fence();
+  }
+  if (warp == 1) tmem_pair_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), 2 * kTileN);
+  pdl_wait();
+  if (warp == 0) {  // the list of tiles: runs of at most kTileN rows of each expert
+    int sum = 0;
+    for (int base = 0; base < a.experts; base += 32) {
+      const int e = base + lane;
+      const int o = e <= a.experts ? a.offsets[e] : 0, next = e < a.experts ? a.offsets[e + 1] : o;
+      int runs = (next - o + kTileN - 1) / kTileN;
+      const int own = runs;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(kAll, runs, d);
+        if (lane >= d) runs += v;
+      }
+      if (e < a.experts) offsets[e] = o, tiles[e] = sum + runs - own;
+      sum += __shfl_sync(kAll, runs, 31);
+    }
+    if (lane == 0) offsets[a.experts] = a.offsets[a.experts], tiles[a.experts] = sum;
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_barrier();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int count = tiles[a.experts] * a.m_tiles, first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+  TileList list = {offsets, tiles, a.m_tiles, 0};
+  uint32_t fault = 0;
+
+  if (warp == 0) {  // producer, in both CTAs: this CTA's half of each operand
+    int s = 0;
+    uint32_t phase = 0;
+    for (int t = first; t < count && !fault; t += stride) {
+      int m, row0, rows;
+      list.at(t, m, row0, rows);
+      const int half = ((rows + 31) & ~31) / 2;  // rows of the N operand in this CTA
+      int gathered[4];
+      if (kGateUp) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // past the run's end: its last row again (those columns are not stored)
+          gathered[i] = a.order[row0 + min((int)rank * half + lane * 4 + i, rows - 1)] / a.top_k;
+      }
+      for (int step = 0; step < a.steps; ++step) {
+        if (!mbar_wait_cluster(empty_bar(s), phase ^ 1)) {  // a fresh barrier counts as freed
+          fault = 2;
+          break;
+        }
+        const uint32_t sa = smem0 + s * kStageBytes, sb = sa + kABytes;
+        const uint32_t bar = cluster_addr(full_bar(s), 0);
+        if (lane == 0) {
+          if (rank == 0) mbar_expect_tx(full_bar(s), 2 * (kABytes + (uint32_t)half * kStepK * 2));
+          if (kGateUp)
+            tma_pair_load5(sa, &maps.a, step * kStepK, 0, 0, m * 8 + rank * 4, list.e, bar);
+          else
+            tma_pair_load3(sa, &maps.a, step * kStepK, m * 256 + rank * 128, list.e, bar);
+        }
+        if (kGateUp) {
+          if (lane * 4 < half) tma_pair_gather4(sb + lane * 512, &maps.b, step * kStepK, gathered, bar);
+        } else if (lane * 16 < half) {
+          tma_pair_load2(sb + lane * 2048, &maps.b, step * kStepK, row0 + rank * half + lane * 16, bar);
+        }
+        if (++s == kStages) s = 0, phase ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {  // one thread of the pair issues the products
+      int s = 0;
+      uint32_t phase = 0;
+      int j = 0;
+      for (int t = first; t < count && !fault; t += stride, ++j) {
+        int m, row0, rows;
+        list.at(t, m, row0, rows);
+        // operand format: 0 = fp16, 1 = bf16, the same for both
+        const uint32_t idesc = umma_idesc(256, (rows + 31) & ~31, false, false) | (a.bf16 ? 1u << 7 | 1u << 10 : 0u);
+        const int acc = j & 1;
+        if (!mbar_wait_cluster(acc_empty(acc), ((j >> 1) & 1) ^ 1)) {
+          fault = 4;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + acc * kTileN;
+        for (int step = 0; step < a.steps; ++step) {
+          if (!mbar_wait_cluster(full_bar(s), phase)) {
+            fault = 1;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t da = smem_desc(smem0 + s * kStageBytes, 16, 1024, kSwizzle128B);
+          const uint64_t db = smem_desc(smem0 + s * kStageBytes + kABytes, 16, 1024, kSwizzle128B);
+#pragma unroll
+          for (int k = 0; k < kStepK / 16; ++k)  // 16 elements: 32 bytes along the swizzled rows
+            umma_pair_ss(d, da + 2 * k, db + 2 * k, idesc, step > 0 || k > 0);
+          umma_pair_commit(empty_bar(s));
+          if (++s == kStages) s = 0, phase ^= 1;
+        }
+        if (!fault) umma_pair_commit(acc_full(acc));
+      }
+    }
+  } else {  // epilogue: TMEM lanes 32 (warp % 4).., every second 32-column chunk
+    const int quarter = warp & 3, group = (warp - 2) >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    unsigned char* own = staging + (warp - 2) * kStagingBytes;
+    int j = 0;
+    for (int t = first; t < count; t += stride, ++j) {
+      int m, row0, rows;
+      list.at(t, m, row0, rows);
+      const int acc = j & 1;
+      if (!mbar_wait_cluster(acc_full(acc), (j >> 1) & 1)) {
+        fault = 4;
+        break;
+      }
+      tc_fence_after();
+      for (int c = group * 32; c < rows; c += 64) {
+        uint32_t r[32];
+        __syncwarp();
+        tmem_ld32(lanes + acc * kTileN + c, r);
+        const int row = row0 + c + lane;  // the row this lane stores
+        if (kGateUp) {
+          const int f0 = m * 128 + (int)rank * 64 + quarter * 16;
+          if (f0 >= a.rows) continue;  // rows is a multiple of 16
+          const bool low = lane < 16;
+          uint16_t* out = reinterpret_cast<uint16_t*>(own) + (low ? 0 : 16) + (lane & 15);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {  // lanes below 16 take column 2i, the others 2i + 1
+            const float even = __uint_as_float(r[2 * i]), odd = __uint_as_float(r[2 * i + 1]);
+            const float other = __shfl_xor_sync(kAll, low ? odd : even, 16);
+            const float g = low ? even : other, u = low ? other : odd;
+            out[i * 32] = T::round(__fdividef(g, 1.0f + __expf(-g)) * u);
+          }
+          __syncwarp();
+          if (c + lane < rows) {
+            const uint4* from = reinterpret_cast<const uint4*>(own + lane * 32);
+            uint4* to = reinterpret_cast<uint4*>(a.h + (int64_t)row * a.rows + f0);
+            to[0] = from[0];
+            to[1] = from[1];
+          }
+          __syncwarp();
+        } else {
+          const int f0 = m * 256 + (int)rank * 128 + quarter * 32;
+          if (f0 >= a.rows) continue;
+          int16_t* out = reinterpret_cast<int16_t*>(own) + lane;
+          float kept = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const uint32_t top = __reduce_max_sync(kAll, r[i] & 0x7fffffffu);
+            const float v = __uint_as_float(r[i]), peak = __uint_as_float(top);
+            float scale;
+            if (peak >= 1e-30f && top < 0x7f800000u) {
+              scale = peak * (1.0f / 32767.0f);
+              out[i * 32] = (int16_t)__float2int_rn(v * __fdividef(32767.0f, peak));
+            } else {  // zeros, vanishing values, infinities, NaN: as bf16
+              scale = -1.0f;
+              out[i * 32] = (int16_t)BF16::round(v);
+            }
+            if (lane == i) kept = scale;
+          }
+          __syncwarp();
+          if (c + lane < rows) {
+            const int64_t pair = a.order[row];
+            const uint4* from = reinterpret_cast<const uint4*>(own + lane * 64);
+            uint4* to = reinterpret_cast<uint4*>(a.share + pair * a.rows + f0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (f0 + i * 8 < a.rows) to[i] = from[i];
+            a.scale[pair * a.blocks + f0 / kShareBlock] = kept;
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty(acc), 0));
+    }
+  }
+  if (fault) {
+    atomicOr(&g_expert_fault, fault);
+    // copies that are still in flight into either CTA land long before this
+    const uint64_t start = global_ns();
+    while (global_ns() - start < 5000000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_barrier();
+  tc_fence_after();
+  if (warp == 1) tmem_pair_dealloc(tmem, 2 * kTileN);
+}
+
+// out[token] = sum of weight * share over the token's choices, in their order; 8 features a thread.
+constexpr int kCombineThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kCombineThreads) expert_combine(ExpertArgs a, const int16_t* __restrict__ share,
+                                                                  const float* __restrict__ scale, int blocks,
+                                                                  FastDiv groups) {
+  pdl_trigger();
+  pdl_wait();
+  const uint32_t i = blockIdx.x * kCombineThreads + threadIdx.x;
+  const uint32_t token = groups.div(i), f = (i - token * groups.d) * 8;
+  if (token >= a.tokens) return;
+  float sum[8] = {};
+#pragma unroll 4
+  for (int j = 0; j < a.top_k; ++j) {
+    const int64_t pair = (int64_t)token * a.top_k + j;
+    if ((unsigned)a.ids[pair] >= (unsigned)a.experts) continue;
+    const float w = a.weights[pair], sc = scale[pair * blocks + f / kShareBlock];
+    const uint4 v = *reinterpret_cast<const uint4*>(share + pair * a.hidden + f);
+    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+    if (sc >= 0.0f) {
+      const float ws = w * sc;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        sum[2 * q] = fmaf(ws, (float)(int16_t)words[q], sum[2 * q]);
+        sum[2 * q + 1] = fmaf(ws, (float)((int32_t)words[q] >> 16), sum[2 * q + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 p = BF16::two(words[q]);
+        sum[2 * q] = fmaf(w, p.x, sum[2 * q]);
+        sum[2 * q + 1] = fmaf(w, p.y, sum[2 * q + 1]);
+      }
+    }
+  }
+  *reinterpret_cast<uint4*>(a.out + token * a.out_stride + f) =
+      make_uint4(T::round2(sum[0], sum[1]), T::round2(sum[2], sum[3]), T::round2(sum[4], sum[5]), T::round2(sum[6], sum[7]));
+}
+
+// Up to this many pairs each pair reads its expert's weights by itself.
+constexpr int64_t kRowsPairs = 32;
+
 struct Sizes {
-  int64_t h, total;
+  int64_t pairs, blocks;
+  bool rows;                                 // the few-pairs kernels
+  int64_t order, h, share, scale, total;     // byte offsets into the workspace (offsets at 0)
 };
 bool sizes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64_t top_k, Sizes* s) {
   if (tokens < 0 || hidden < 1 || inner < 1 || experts < 1 || experts > kMaxExperts || top_k < 1 ||
       top_k > kMaxChoices || tokens > INT32_MAX / 256 / top_k || hidden > (1 << 20) || inner > (1 << 20))
     return false;
-  const int64_t pairs = tokens * top_k;
-  s->h = 0;
-  s->total = (pairs * inner * 4 + 255) / 256 * 256;
+  auto pad = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
+  s->pairs = tokens * top_k;
+  s->blocks = (hidden + kShareBlock - 1) / kShareBlock;
+  s->rows = s->pairs <= kRowsPairs;
+  if (s->rows) {
+    s->order = s->h = s->share = s->scale = 0;
+    s->total = pad(s->pairs * inner * 4);
+  } else {
+    s->order = pad((experts + 1) * 4);
+    s->h = s->order + pad(s->pairs * 4);
+    s->share = s->h + pad(s->pairs * inner * 2);
+    s->scale = s->share + pad(s->pairs * hidden * 2);
+    s->total = s->scale + pad(s->pairs * s->blocks * 4);
+  }
   return true;
 }
 
+ttn_status encode_map(const char* name, CUtensorMap* map, bool bf16, int rank, const void* base, const cuuint64_t* dims,
+                      const cuuint64_t* strides, const cuuint32_t* box) {
+  const auto encode = tensor_map_encoder();
+  if (!encode) return fail(TTN_CUDA_ERROR, "%s: cuTensorMapEncodeTiled is not available", name);
+  const cuuint32_t unit[5] = {1, 1, 1, 1, 1};
+  const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                            (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, unit,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TTN_UNSUPPORTED, "%s: cuTensorMapEncodeTiled %d", name, (int)r);
+  return TTN_OK;
+}
+
 template <typename T>
-ttn_status launch_experts(const char* name, const ExpertArgs& a, void* workspace, cudaStream_t stream) {
+ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s, unsigned char* ws, cudaStream_t stream) {
+  constexpr bool bf16 = std::is_same<T, BF16>::value;
+  int32_t *offsets = (int32_t*)ws, *order = (int32_t*)(ws + s.order);
+  uint16_t* h = (uint16_t*)(ws + s.h);
+  int16_t* share = (int16_t*)(ws + s.share);
+  float* scale = (float*)(ws + s.scale);
+  const cuuint64_t hidden = a.hidden, inner = a.inner, experts = a.experts;
+  ProductMaps gate, down;
+  {  // gate-up weights: (hidden, 16 rows, gate | up, inner / 16, expert)
+    const cuuint64_t dims[5] = {hidden, 16, 2, inner / 16, experts};
+    const cuuint64_t str[4] = {hidden * 2, inner * hidden * 2, 16 * hidden * 2, 2 * inner * hidden * 2};
+    const cuuint32_t box[5] = {kStepK, 16, 2, 4, 1};
+    TTN_TRY(encode_map(name, &gate.a, bf16, 5, a.gate_up, dims, str, box));
+  }
+  {  // x: one row a box, four rows a gather
+    const cuuint64_t dims[2] = {hidden, (cuuint64_t)a.tokens};
+    const cuuint64_t str[1] = {(cuuint64_t)a.x_stride * 2};
+    const cuuint32_t box[2] = {kStepK, 1};
+    TTN_TRY(encode_map(name, &gate.b, bf16, 2, a.x, dims, str, box));
+  }
+  {
+    const cuuint64_t dims[3] = {inner, hidden, experts};
+    const cuuint64_t str[2] = {inner * 2, hidden * inner * 2};
+    const cuuint32_t box[3] = {kStepK, 128, 1};
+    TTN_TRY(encode_map(name, &down.a, bf16, 3, a.down, dims, str, box));
+  }
+  {
+    const cuuint64_t dims[2] = {inner, (cuuint64_t)s.pairs};
+    const cuuint64_t str[1] = {inner * 2};
+    const cuuint32_t box[2] = {kStepK, 16};
+    TTN_TRY(encode_map(name, &down.b, bf16, 2, h, dims, str, box));
+  }
+  TTN_TRY(cuda_check(launch_pdl(expert_plan, dim3((unsigned)a.experts), dim3(kPlanThreads), 0, stream, a.ids,
+                                (int)s.pairs, a.experts, offsets, order),
+                     name));
+  const int64_t runs = s.pairs / kTileN + (s.pairs < a.experts ? s.pairs : a.experts);  // at most
+  const uint32_t smem = product_smem(a.experts);
+  auto products = [&](auto kernel, const ProductMaps& maps, int rows, int length, int tile) {
+    ProductArgs p = {};
+    p.offsets = offsets, p.order = order, p.h = h, p.share = share, p.scale = scale;
+    p.experts = a.experts, p.top_k = a.top_k, p.rows = rows;
+    p.steps = (length + kStepK - 1) / kStepK;
+    p.m_tiles = (rows + tile - 1) / tile;
+    p.blocks = (int)s.blocks;
+    p.bf16 = bf16;
+    if (runs * p.m_tiles > INT32_MAX) return fail(TTN_UNSUPPORTED, "%s: more than 2^31 tiles", name);
+    TTN_TRY(ensure_dynamic_smem((const void*)kernel, (int)smem));
+    const int64_t pairs_of_sms = sm_count() / 2, most = runs * p.m_tiles;
+    const unsigned grid = 2 * (unsigned)(most < pairs_of_sms ? most : pairs_of_sms);
+    return cuda_check(launch_pdl(kernel, dim3(grid), dim3(kProductThreads), smem, stream, p, maps), name);
+  };
+  TTN_TRY(products(expert_products<T, true>, gate, a.inner, a.hidden, 128));
+  TTN_TRY(products(expert_products<T, false>, down, a.hidden, a.inner, 256));
+  const int64_t items = a.tokens * (a.hidden / 8);
+  if (items + kCombineThreads > UINT32_MAX) return fail(TTN_UNSUPPORTED, "%s: output too large", name);
+  return cuda_check(launch_pdl(expert_combine<T>, dim3((unsigned)((items + kCombineThreads - 1) / kCombineThreads)),
+                               dim3(kCombineThreads), 0, stream, a, (const int16_t*)share, (const float*)scale,
+                               (int)s.blocks, FastDiv((uint32_t)(a.hidden / 8))),
+                    name);
+}
+
+template <typename T>
+ttn_status launch_experts(const char* name, const ExpertArgs& a, const Sizes& s, void* workspace, cudaStream_t stream) {
+  if (!s.rows) return launch_products<T>(name, a, s, (unsigned char*)workspace, stream);
   float* h = (float*)workspace;
-  const int64_t pairs = a.tokens * a.top_k;
+  const int64_t pairs = s.pairs;
   const int gate_blocks = (a.inner + kRowsBlock - 1) / kRowsBlock, down_blocks = a.hidden / kDownRows;
   if (pairs * gate_blocks > INT32_MAX || a.tokens * down_blocks > INT32_MAX)
     return fail(TTN_UNSUPPORTED, "%s: too many tokens for these sizes", name);
@@ -204,8 +664,16 @@ ttn_status ttn_expert_mlp(int dtype, const void* x, int64_t x_row_stride, int64_
   a.out_stride = tokens > 1 ? out_row_stride : hidden;
   a.tokens = tokens;
   a.hidden = (int)hidden, a.inner = (int)inner, a.experts = (int)num_experts, a.top_k = (int)top_k;
-  return dtype == TTN_F16 ? launch_experts<F16>(name, a, workspace, (cudaStream_t)stream)
-                          : launch_experts<BF16>(name, a, workspace, (cudaStream_t)stream);
+  return dtype == TTN_F16 ? launch_experts<F16>(name, a, s, workspace, (cudaStream_t)stream)
+                          : launch_experts<BF16>(name, a, s, workspace, (cudaStream_t)stream);
+}
+
+ttn_status ttn_expert_mlp_fault(uint32_t* fault) {
+  const char* name = "ttn_expert_mlp_fault";
+  if (!fault) return fail(TTN_INVALID_ARG, "%s: null pointer", name);
+  TTN_TRY(cuda_check(cudaMemcpyFromSymbol(fault, g_expert_fault, sizeof(uint32_t)), name));
+  const uint32_t zero = 0;
+  return cuda_check(cudaMemcpyToSymbol(g_expert_fault, &zero, sizeof(zero)), name);
 }
 
 }  // extern "C"

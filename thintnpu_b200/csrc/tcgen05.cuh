@@ -160,6 +160,99 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols));
 }
 
+// ---- pairs of CTAs (clusters of two, cta_group::2): rank 0 leads and issues the products
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address, in the cluster's shared-memory window, of `saddr` in CTA `rank`.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_mbar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_mbar) : "memory");
+}
+// mbar_wait for a barrier that the other CTA of the pair signals too.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t mbar, uint32_t phase) {
+  const uint64_t start = global_ns();
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(mbar), "r"(phase)
+        : "memory");
+    if (done) return true;
+    if (global_ns() - start > kWaitNs) return false;
+  }
+}
+// Tile loads into this CTA's shared memory, completing on a barrier of either CTA of the
+// pair (`cluster_mbar` from cluster_addr).
+__device__ __forceinline__ void tma_pair_load2(uint32_t dst, const CUtensorMap* map, int c0, int c1,
+                                               uint32_t cluster_mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(cluster_mbar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_pair_load3(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                               uint32_t cluster_mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
+      "%4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(cluster_mbar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_pair_load5(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                               int c4, uint32_t cluster_mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, "
+      "%4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(cluster_mbar)
+      : "memory");
+}
+// Four rows of a 2-D map with boxes one row high, at column c0.
+__device__ __forceinline__ void tma_pair_gather4(uint32_t dst, const CUtensorMap* map, int c0, const int (&row)[4],
+                                                 uint32_t cluster_mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+      "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]),
+      "r"(cluster_mbar)
+      : "memory");
+}
+// D (both CTAs' TMEM, half of the M rows each) [+]= A (half of the rows in each CTA) x B
+// (half of the columns in each CTA); one thread of the leader.
+__device__ __forceinline__ void umma_pair_ss(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc));
+}
+// Arrives on the barrier at this offset in both CTAs once the products issued so far are done.
+__device__ __forceinline__ void umma_pair_commit(uint32_t mbar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(mbar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_pair_alloc(uint32_t slot, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols));
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+}
+__device__ __forceinline__ void tmem_pair_dealloc(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols));
+}
+
 }  // namespace tc
 
 // Host: the driver's cuTensorMapEncodeTiled, looked up once (nullptr if unavailable).

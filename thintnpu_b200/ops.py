@@ -730,6 +730,13 @@ def expert_mlp(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, ga
     return out
 
 
+def expert_mlp_fault() -> int:
+    """Reads and clears the experts' products' fault word (0 = no launch gave up)."""
+    word = ctypes.c_uint32(0)
+    call("ttn_expert_mlp_fault", ctypes.byref(word))
+    return int(word.value)
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, scale: float = 1.0):
     """Log probabilities of given tokens under ``softmax(scale * logits)``:
     ``(logprobs [rows], entropy [rows], top_logprobs [rows, top], top_tokens [rows, top])``,
