@@ -12,6 +12,7 @@
 //    32), so an expert with few rows costs few columns, and a batch of single tokens
 //    streams each expert's weights once through tiles 32 columns wide.
 //    - The rows of x are gathered by TMA (tile::gather4) through `order`: no sorted copy.
+//      Four threads of four warps issue the copies, with their rows in registers.
 //    - A CTA's 128 weight rows of the first product are 4 x (16 gate rows, 16 up rows),
 //      one TMA box of a five-dimensional map, so that the gate and up values of a feature
 //      sit in lanes l and l + 16 of one warp: one shuffle a value pair, then
@@ -156,44 +157,72 @@ __global__ void __launch_bounds__(kDownWarps * 32) expert_rows_down(ExpertArgs a
 __device__ uint32_t g_expert_fault;
 
 // offsets[e]: pairs of experts below e; order: the pairs, by expert, then by number.  One
-// block an expert, each reading all ids (they are few and in L2): no block waits for another.
-constexpr int kPlanThreads = 512;
+// block an expert, each reading all ids twice (they are few and in L2), 128 a warp and load:
+// no block waits for another.  65,536 ids of 64 experts take 8 us on a B200.
+constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanBatch = 4;  // loads in flight
 __global__ void __launch_bounds__(kPlanThreads) expert_plan(const int32_t* __restrict__ ids, int pairs, int experts,
-                                                            int32_t* __restrict__ offsets, int32_t* __restrict__ order) {
+                                                            int vec, int32_t* __restrict__ offsets,
+                                                            int32_t* __restrict__ order) {
   __shared__ int below[kPlanWarps], mine[kPlanWarps];
   pdl_trigger();
   pdl_wait();
   const int e = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int chunk = (pairs + kPlanWarps * 32 - 1) / (kPlanWarps * 32) * 32;
-  const int64_t first = (int64_t)warp * chunk;
-  const int64_t last = first + chunk < pairs ? first + chunk : pairs;
+  const int chunk = (pairs + kPlanWarps * 128 - 1) / (kPlanWarps * 128) * 128;  // ids of one warp
+  const int first = warp * chunk, last = min(first + chunk, pairs);            // pairs < 2^23
+  auto load = [&](int i0, int (&id)[4]) {
+    const int i = i0 + lane * 4;
+    if (vec && i + 4 <= last) {
+      const int4 v = __ldg(reinterpret_cast<const int4*>(ids + i));
+      id[0] = v.x, id[1] = v.y, id[2] = v.z, id[3] = v.w;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) id[q] = i + q < last ? ids[i + q] : -1;
+    }
+  };
   int less = 0, equal = 0;
-  for (int64_t i = first + lane; i < last; i += 32) {
-    const int id = ids[i];
-    less += (unsigned)id < (unsigned)e;
-    equal += id == e;
+  for (int i0 = first; i0 < last; i0 += 128 * kPlanBatch) {
+    int id[kPlanBatch][4];
+#pragma unroll
+    for (int u = 0; u < kPlanBatch; ++u) load(i0 + u * 128, id[u]);
+#pragma unroll
+    for (int u = 0; u < kPlanBatch; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) less += (unsigned)id[u][q] < (unsigned)e, equal += id[u][q] == e;
   }
   less = __reduce_add_sync(kAll, less);
   equal = __reduce_add_sync(kAll, equal);
   if (lane == 0) below[warp] = less, mine[warp] = equal;
   __syncthreads();
-  int at = 0, total = 0;
-  for (int w = 0; w < kPlanWarps; ++w) {
-    at += below[w] + (w < warp ? mine[w] : 0);
-    total += below[w] + mine[w];
-  }
+  static_assert(kPlanWarps == 32, "one lane a warp");
+  const int total = __reduce_add_sync(kAll, below[lane]);
+  int at = total + __reduce_add_sync(kAll, lane < warp ? mine[lane] : 0);
+  const int all = total + __reduce_add_sync(kAll, mine[lane]);
   if (threadIdx.x == 0) {
-    offsets[e] = at;  // warp 0: nothing of this expert before it
-    if (e == experts - 1) offsets[experts] = total;
+    offsets[e] = total;
+    if (e == experts - 1) offsets[experts] = all;
   }
   if (!equal) return;
-  for (int64_t i0 = first; i0 < last; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const bool in = i < last && ids[i] == e;
-    const uint32_t vote = __ballot_sync(kAll, in);
-    if (in) order[at + __popc(vote & ((1u << lane) - 1))] = (int)i;
-    at += __popc(vote);
+  const uint32_t before = (1u << lane) - 1;
+  for (int i0 = first; i0 < last; i0 += 128 * kPlanBatch) {
+    int id[kPlanBatch][4];
+#pragma unroll
+    for (int u = 0; u < kPlanBatch; ++u) load(i0 + u * 128, id[u]);
+#pragma unroll
+    for (int u = 0; u < kPlanBatch; ++u) {
+      int seen = 0, ahead = 0;  // of this load: all lanes', the lower lanes'
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t vote = __ballot_sync(kAll, id[u][q] == e);
+        seen += __popc(vote);
+        ahead += __popc(vote & before);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (id[u][q] == e) order[at + ahead++] = i0 + u * 128 + lane * 4 + q;
+      at += seen;
+    }
   }
 }
 
@@ -203,7 +232,9 @@ constexpr int kStages = 6;
 constexpr uint32_t kABytes = 128 * kStepK * 2, kBBytes = kTileN / 2 * kStepK * 2;
 constexpr uint32_t kStageBytes = kABytes + kBBytes;
 constexpr int kEpiWarps = 8;
-constexpr int kProductThreads = 64 + 32 * kEpiWarps;
+constexpr int kGatherWarps = 4;  // of the first product
+constexpr int kGatherRows = kTileN / 2 / kGatherWarps;
+constexpr int product_threads(bool gate_up) { return 64 + 32 * kEpiWarps + (gate_up ? 32 * kGatherWarps : 0); }
 constexpr uint32_t kStagingBytes = 32 * 64;  // one epilogue warp: 32 rows x 64 bytes
 constexpr int kShareBlock = 32;              // features that share a scale
 
@@ -240,7 +271,7 @@ struct TileList {
 };
 
 template <typename T, bool kGateUp>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGateUp), 1)
     expert_products(ProductArgs a, const __grid_constant__ ProductMaps maps) {
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[2 * kStages + 4];  // full[s], empty[s], acc_full[2], acc_empty[2]
@@ -298,43 +329,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
   TileList list = {offsets, tiles, a.m_tiles, 0};
   uint32_t fault = 0;
 
-  if (warp == 0) {  // producer, in both CTAs: this CTA's half of each operand
+  if (warp == 0) {  // producer, in both CTAs: this CTA's half of the operands that TMA loads
     int s = 0;
     uint32_t phase = 0;
     for (int t = first; t < count && !fault; t += stride) {
       int m, row0, rows;
       list.at(t, m, row0, rows);
       const int half = ((rows + 31) & ~31) / 2;  // rows of the N operand in this CTA
-      int gathered[4];
-      if (kGateUp) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)  // past the run's end: its last row again (those columns are not stored)
-          gathered[i] = a.order[row0 + min((int)rank * half + lane * 4 + i, rows - 1)] / a.top_k;
-      }
       for (int step = 0; step < a.steps; ++step) {
-        if (!mbar_wait_cluster(empty_bar(s), phase ^ 1)) {  // a fresh barrier counts as freed
+        // a fresh barrier counts as freed; the vote keeps the lanes within one step of each other
+        if (!__all_sync(kAll, mbar_wait_cluster<true>(empty_bar(s), phase ^ 1))) {
           fault = 2;
           break;
         }
         const uint32_t sa = smem0 + s * kStageBytes, sb = sa + kABytes;
         const uint32_t bar = cluster_addr(full_bar(s), 0);
-        if (lane == 0) {
+        if (elect_one()) {
           if (rank == 0) mbar_expect_tx(full_bar(s), 2 * (kABytes + (uint32_t)half * kStepK * 2));
-          if (kGateUp)
+          if (kGateUp) {
             tma_pair_load5(sa, &maps.a, step * kStepK, 0, 0, m * 8 + rank * 4, list.e, bar);
-          else
+          } else {
             tma_pair_load3(sa, &maps.a, step * kStepK, m * 256 + rank * 128, list.e, bar);
+#pragma unroll
+            for (int i = 0; i < kTileN / 32; ++i)
+              if (i * 16 < half)
+                tma_pair_load2(sb + i * 2048, &maps.b, step * kStepK, row0 + rank * half + i * 16, bar);
+          }
         }
-        if (kGateUp) {
-          if (lane * 4 < half) tma_pair_gather4(sb + lane * 512, &maps.b, step * kStepK, gathered, bar);
-        } else if (lane * 16 < half) {
-          tma_pair_load2(sb + lane * 2048, &maps.b, step * kStepK, row0 + rank * half + lane * 16, bar);
+        __syncwarp();
+        if (++s == kStages) s = 0, phase ^= 1;
+      }
+    }
+  } else if (kGateUp && warp >= 2 + kEpiWarps) {
+    // Gathering warps, one thread each: every fourth copy of four rows.  A stage has 16 rows at
+    // least, so each warp has a part in every stage: none falls two phases of a barrier
+    // behind, where parities repeat.
+    const int line = (warp - 2 - kEpiWarps) * 4;
+    int s = 0;
+    uint32_t phase = 0;
+    for (int t = first; t < count && !fault; t += stride) {
+      int m, row0, rows;
+      list.at(t, m, row0, rows);
+      const int half = ((rows + 31) & ~31) / 2;
+      int from[kGatherRows / 4][4];
+#pragma unroll
+      for (int i = 0; i < kGatherRows; ++i) {  // past the run's end: its last row (those columns are not stored)
+        const int row = (int)rank * half + line + i / 4 * (4 * kGatherWarps) + i % 4;
+        from[i / 4][i % 4] = a.order[row0 + min(row, rows - 1)] / a.top_k;
+      }
+      for (int step = 0; step < a.steps; ++step) {
+        if (!__all_sync(kAll, mbar_wait_cluster<true>(empty_bar(s), phase ^ 1))) {
+          fault = 2;
+          break;
         }
+        const uint32_t sb = smem0 + s * kStageBytes + kABytes + line * kStepK * 2;
+        const uint32_t bar = cluster_addr(full_bar(s), 0);
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < kGatherRows / 4; ++i)
+            if (line + i * 4 * kGatherWarps < half)
+              tma_pair_gather4(sb + i * 512 * kGatherWarps, &maps.b, step * kStepK, from[i], bar);
+        }
+        __syncwarp();
         if (++s == kStages) s = 0, phase ^= 1;
       }
     }
   } else if (warp == 1) {
-    if (rank == 0 && lane == 0) {  // one thread of the pair issues the products
+    if (rank == 0) {  // one thread of the pair issues the products
       int s = 0;
       uint32_t phase = 0;
       int j = 0;
@@ -344,30 +405,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         // operand format: 0 = fp16, 1 = bf16, the same for both
         const uint32_t idesc = umma_idesc(256, (rows + 31) & ~31, false, false) | (a.bf16 ? 1u << 7 | 1u << 10 : 0u);
         const int acc = j & 1;
-        if (!mbar_wait_cluster(acc_empty(acc), ((j >> 1) & 1) ^ 1)) {
+        if (!__all_sync(kAll, mbar_wait_cluster<true>(acc_empty(acc), ((j >> 1) & 1) ^ 1))) {
           fault = 4;
           break;
         }
-        tc_fence_after();
         const uint32_t d = tmem + acc * kTileN;
         for (int step = 0; step < a.steps; ++step) {
-          if (!mbar_wait_cluster(full_bar(s), phase)) {
+          if (!__all_sync(kAll, mbar_wait_cluster<true>(full_bar(s), phase))) {
             fault = 1;
             break;
           }
           tc_fence_after();
           const uint64_t da = smem_desc(smem0 + s * kStageBytes, 16, 1024, kSwizzle128B);
           const uint64_t db = smem_desc(smem0 + s * kStageBytes + kABytes, 16, 1024, kSwizzle128B);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kStepK / 16; ++k)  // 16 elements: 32 bytes along the swizzled rows
-            umma_pair_ss(d, da + 2 * k, db + 2 * k, idesc, step > 0 || k > 0);
-          umma_pair_commit(empty_bar(s));
+            for (int k = 0; k < kStepK / 16; ++k)  // 16 elements: 32 bytes along the swizzled rows
+              umma_pair_ss(d, da + 2 * k, db + 2 * k, idesc, step > 0 || k > 0);
+            umma_pair_commit(empty_bar(s));
+            if (step == a.steps - 1) umma_pair_commit(acc_full(acc));
+          }
+          __syncwarp();
           if (++s == kStages) s = 0, phase ^= 1;
         }
-        if (!fault) umma_pair_commit(acc_full(acc));
       }
     }
-  } else {  // epilogue: TMEM lanes 32 (warp % 4).., every second 32-column chunk
+  } else if (warp < 2 + kEpiWarps) {  // epilogue: TMEM lanes 32 (warp % 4).., every second 32-column chunk
     const int quarter = warp & 3, group = (warp - 2) >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     unsigned char* own = staging + (warp - 2) * kStagingBytes;
@@ -376,7 +439,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
       int m, row0, rows;
       list.at(t, m, row0, rows);
       const int acc = j & 1;
-      if (!mbar_wait_cluster(acc_full(acc), (j >> 1) & 1)) {
+      if (!__all_sync(kAll, mbar_wait_cluster<false>(acc_full(acc), (j >> 1) & 1))) {
         fault = 4;
         break;
       }
@@ -385,7 +448,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
         uint32_t r[32];
         __syncwarp();
         tmem_ld32(lanes + acc * kTileN + c, r);
-        const int row = row0 + c + lane;  // the row this lane stores
         if (kGateUp) {
           const int f0 = m * 128 + (int)rank * 64 + quarter * 16;
           if (f0 >= a.rows) continue;  // rows is a multiple of 16
@@ -399,11 +461,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
             out[i * 32] = T::round(__fdividef(g, 1.0f + __expf(-g)) * u);
           }
           __syncwarp();
-          if (c + lane < rows) {
-            const uint4* from = reinterpret_cast<const uint4*>(own + lane * 32);
-            uint4* to = reinterpret_cast<uint4*>(a.h + (int64_t)row * a.rows + f0);
-            to[0] = from[0];
-            to[1] = from[1];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {  // two lanes a row: whole 32-byte sectors
+            const int n = i * 16 + (lane >> 1), q = lane & 1;
+            if (c + n < rows)
+              reinterpret_cast<uint4*>(a.h + (int64_t)(row0 + c + n) * a.rows + f0)[q] =
+                  reinterpret_cast<const uint4*>(own)[n * 2 + q];
           }
           __syncwarp();
         } else {
@@ -426,14 +489,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
             if (lane == i) kept = scale;
           }
           __syncwarp();
-          if (c + lane < rows) {
-            const int64_t pair = a.order[row];
-            const uint4* from = reinterpret_cast<const uint4*>(own + lane * 64);
-            uint4* to = reinterpret_cast<uint4*>(a.share + pair * a.rows + f0);
+          const int pair = c + lane < rows ? a.order[row0 + c + lane] : -1;
+          if (pair >= 0) a.scale[(int64_t)pair * a.blocks + f0 / kShareBlock] = kept;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (f0 + i * 8 < a.rows) to[i] = from[i];
-            a.scale[pair * a.blocks + f0 / kShareBlock] = kept;
+          for (int i = 0; i < 4; ++i) {  // four lanes a row: 64 contiguous bytes
+            const int n = i * 8 + (lane >> 2), q = lane & 3;
+            const int to = __shfl_sync(kAll, pair, n);
+            if (to >= 0 && f0 + q * 8 < a.rows)
+              reinterpret_cast<uint4*>(a.share + (int64_t)to * a.rows + f0)[q] =
+                  reinterpret_cast<const uint4*>(own)[n * 4 + q];
           }
           __syncwarp();
         }
@@ -468,26 +532,37 @@ __global__ void __launch_bounds__(kCombineThreads) expert_combine(ExpertArgs a, 
   const uint32_t token = groups.div(i), f = (i - token * groups.d) * 8;
   if (token >= a.tokens) return;
   float sum[8] = {};
-#pragma unroll 4
-  for (int j = 0; j < a.top_k; ++j) {
-    const int64_t pair = (int64_t)token * a.top_k + j;
-    if ((unsigned)a.ids[pair] >= (unsigned)a.experts) continue;
-    const float w = a.weights[pair], sc = scale[pair * blocks + f / kShareBlock];
-    const uint4 v = *reinterpret_cast<const uint4*>(share + pair * a.hidden + f);
-    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-    if (sc >= 0.0f) {
-      const float ws = w * sc;
+  constexpr int kBatch = 8;  // choices whose loads are in flight together
+  for (int j0 = 0; j0 < a.top_k; j0 += kBatch) {
+    const int64_t pair0 = (int64_t)token * a.top_k + j0;
+    float w[kBatch], sc[kBatch];
+    uint4 v[kBatch];
+    bool live[kBatch];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        sum[2 * q] = fmaf(ws, (float)(int16_t)words[q], sum[2 * q]);
-        sum[2 * q + 1] = fmaf(ws, (float)((int32_t)words[q] >> 16), sum[2 * q + 1]);
-      }
-    } else {
+    for (int j = 0; j < kBatch; ++j) {  // shares of pairs without an expert were never written
+      live[j] = j0 + j < a.top_k && (unsigned)a.ids[pair0 + j] < (unsigned)a.experts;
+      w[j] = live[j] ? a.weights[pair0 + j] : 0.0f;
+      sc[j] = live[j] ? scale[(pair0 + j) * blocks + f / kShareBlock] : 0.0f;
+      v[j] = live[j] ? *reinterpret_cast<const uint4*>(share + (pair0 + j) * a.hidden + f) : make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float2 p = BF16::two(words[q]);
-        sum[2 * q] = fmaf(w, p.x, sum[2 * q]);
-        sum[2 * q + 1] = fmaf(w, p.y, sum[2 * q + 1]);
+    for (int j = 0; j < kBatch; ++j) {
+      if (!live[j]) continue;
+      const uint32_t words[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+      if (sc[j] >= 0.0f) {
+        const float ws = w[j] * sc[j];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          sum[2 * q] = fmaf(ws, (float)(int16_t)words[q], sum[2 * q]);
+          sum[2 * q + 1] = fmaf(ws, (float)((int32_t)words[q] >> 16), sum[2 * q + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 p = BF16::two(words[q]);
+          sum[2 * q] = fmaf(w[j], p.x, sum[2 * q]);
+          sum[2 * q + 1] = fmaf(w[j], p.y, sum[2 * q + 1]);
+        }
       }
     }
   }
@@ -571,11 +646,11 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     TTN_TRY(encode_map(name, &down.b, bf16, 2, h, dims, str, box));
   }
   TTN_TRY(cuda_check(launch_pdl(expert_plan, dim3((unsigned)a.experts), dim3(kPlanThreads), 0, stream, a.ids,
-                                (int)s.pairs, a.experts, offsets, order),
+                                (int)s.pairs, a.experts, (int)((uintptr_t)a.ids % 16 == 0), offsets, order),
                      name));
   const int64_t runs = s.pairs / kTileN + (s.pairs < a.experts ? s.pairs : a.experts);  // at most
   const uint32_t smem = product_smem(a.experts);
-  auto products = [&](auto kernel, const ProductMaps& maps, int rows, int length, int tile) {
+  auto products = [&](auto kernel, const ProductMaps& maps, int rows, int length, int tile, int threads) {
     ProductArgs p = {};
     p.offsets = offsets, p.order = order, p.h = h, p.share = share, p.scale = scale;
     p.experts = a.experts, p.top_k = a.top_k, p.rows = rows;
@@ -587,10 +662,10 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     TTN_TRY(ensure_dynamic_smem((const void*)kernel, (int)smem));
     const int64_t pairs_of_sms = sm_count() / 2, most = runs * p.m_tiles;
     const unsigned grid = 2 * (unsigned)(most < pairs_of_sms ? most : pairs_of_sms);
-    return cuda_check(launch_pdl(kernel, dim3(grid), dim3(kProductThreads), smem, stream, p, maps), name);
+    return cuda_check(launch_pdl(kernel, dim3(grid), dim3(threads), smem, stream, p, maps), name);
   };
-  TTN_TRY(products(expert_products<T, true>, gate, a.inner, a.hidden, 128));
-  TTN_TRY(products(expert_products<T, false>, down, a.hidden, a.inner, 256));
+  TTN_TRY(products(expert_products<T, true>, gate, a.inner, a.hidden, 128, product_threads(true)));
+  TTN_TRY(products(expert_products<T, false>, down, a.hidden, a.inner, 256, product_threads(false)));
   const int64_t items = a.tokens * (a.hidden / 8);
   if (items + kCombineThreads > UINT32_MAX) return fail(TTN_UNSUPPORTED, "%s: output too large", name);
   return cuda_check(launch_pdl(expert_combine<T>, dim3((unsigned)((items + kCombineThreads - 1) / kCombineThreads)),

@@ -170,6 +170,17 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// True in one lane of a converged warp, always the same one.  Code under elect_one() is known
+// to the compiler to run in a single thread; under any other condition it guards the uniform
+// operands of each TMA, tcgen05.mma and commit against lanes that disagree, about 130 cycles
+// an instruction, executed or not.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(one));
+  return one != 0;
+}
 // The address, in the cluster's shared-memory window, of `saddr` in CTA `rank`.
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) {
   uint32_t r;
@@ -179,19 +190,34 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) 
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_mbar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_mbar) : "memory");
 }
-// mbar_wait for a barrier that the other CTA of the pair signals too.
+// mbar_wait for a barrier that the other CTA of the pair signals too.  kPoll: test_wait, which
+// does not suspend the thread, for the roles that every stage waits for.  The wall clock is
+// read only once a wait has failed a number of times: in a running pipeline most do not.
+template <bool kPoll>
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t mbar, uint32_t phase) {
-  const uint64_t start = global_ns();
-  while (true) {
+  uint64_t start = 0;
+  for (uint32_t tries = 1;; ++tries) {
     uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(done)
-        : "r"(mbar), "r"(phase)
-        : "memory");
+    if (kPoll)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.b32 %0, 1, 0, p;\n\t}\n"
+          : "=r"(done)
+          : "r"(mbar), "r"(phase)
+          : "memory");
+    else
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.b32 %0, 1, 0, p;\n\t}\n"
+          : "=r"(done)
+          : "r"(mbar), "r"(phase)
+          : "memory");
     if (done) return true;
-    if (global_ns() - start > kWaitNs) return false;
+    if ((tries & (kPoll ? 255u : 15u)) == 0u) {
+      const uint64_t now = global_ns();
+      if (!start) start = now;
+      if (now - start > kWaitNs) return false;
+    }
   }
 }
 // Tile loads into this CTA's shared memory, completing on a barrier of either CTA of the
