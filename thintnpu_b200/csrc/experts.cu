@@ -234,8 +234,9 @@ constexpr uint32_t kStageBytes = kABytes + kBBytes;
 constexpr int kEpiWarps = 8;
 constexpr int kGatherWarps = 4;  // of the first product
 constexpr int kGatherRows = kTileN / 2 / kGatherWarps;
-constexpr int product_threads(bool gate_up) { return 64 + 32 * kEpiWarps + (gate_up ? 32 * kGatherWarps : 0); }
-constexpr uint32_t kStagingBytes = 32 * 64;  // one epilogue warp: 32 rows x 64 bytes
+constexpr int product_threads(bool gather) { return 64 + 32 * kEpiWarps + (gather ? 32 * kGatherWarps : 0); }
+constexpr int kStagingPitch = 36;                          // words: conflict-free both ways
+constexpr uint32_t kStagingBytes = 16 * kStagingPitch * 4;  // one epilogue warp: 16 rows x 32 values (or 32 x 16 halves)
 constexpr int kShareBlock = 32;              // features that share a scale
 
 struct ProductArgs {
@@ -245,6 +246,7 @@ struct ProductArgs {
   float* scale;     // down: [pair][blocks]
   int experts, top_k, rows, steps, m_tiles, blocks;  // rows: weight rows of the product (inner or hidden)
   int bf16;
+  int wide;         // down: share rows are multiples of 32 bytes
 };
 struct ProductMaps {
   CUtensorMap a, b;
@@ -270,8 +272,9 @@ struct TileList {
   }
 };
 
-template <typename T, bool kGateUp>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGateUp), 1)
+// kGateUp: the first product; kGather: its token rows come from x through `order` (else from a sorted copy).
+template <typename T, bool kGateUp, bool kGather>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGather), 1)
     expert_products(ProductArgs a, const __grid_constant__ ProductMaps maps) {
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[2 * kStages + 4];  // full[s], empty[s], acc_full[2], acc_empty[2]
@@ -346,10 +349,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
         const uint32_t bar = cluster_addr(full_bar(s), 0);
         if (elect_one()) {
           if (rank == 0) mbar_expect_tx(full_bar(s), 2 * (kABytes + (uint32_t)half * kStepK * 2));
-          if (kGateUp) {
+          if (kGateUp)
             tma_pair_load5(sa, &maps.a, step * kStepK, 0, 0, m * 8 + rank * 4, list.e, bar);
-          } else {
+          else
             tma_pair_load3(sa, &maps.a, step * kStepK, m * 256 + rank * 128, list.e, bar);
+          if (!kGather) {
 #pragma unroll
             for (int i = 0; i < kTileN / 32; ++i)
               if (i * 16 < half)
@@ -360,7 +364,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
         if (++s == kStages) s = 0, phase ^= 1;
       }
     }
-  } else if (kGateUp && warp >= 2 + kEpiWarps) {
+  } else if (kGather && warp >= 2 + kEpiWarps) {
     // Gathering warps, one thread each: every fourth copy of four rows.  A stage has 16 rows at
     // least, so each warp has a part in every stage: none falls two phases of a barrier
     // behind, where parities repeat.
@@ -444,15 +448,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
         break;
       }
       tc_fence_after();
-      for (int c = group * 32; c < rows; c += 64) {
-        uint32_t r[32];
-        __syncwarp();
-        tmem_ld32(lanes + acc * kTileN + c, r);
-        if (kGateUp) {
-          const int f0 = m * 128 + (int)rank * 64 + quarter * 16;
-          if (f0 >= a.rows) continue;  // rows is a multiple of 16
-          const bool low = lane < 16;
-          uint16_t* out = reinterpret_cast<uint16_t*>(own) + (low ? 0 : 16) + (lane & 15);
+      if (kGateUp) {
+        const int f0 = m * 128 + (int)rank * 64 + quarter * 16;
+        const bool low = lane < 16;
+        uint16_t* out = reinterpret_cast<uint16_t*>(own) + (low ? 0 : 16) + (lane & 15);
+        for (int c = group * 32; c < rows && f0 < a.rows; c += 64) {  // a.rows is a multiple of 16
+          uint32_t r[32];
+          tmem_ld32(lanes + acc * kTileN + c, r);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {  // lanes below 16 take column 2i, the others 2i + 1
             const float even = __uint_as_float(r[2 * i]), odd = __uint_as_float(r[2 * i + 1]);
@@ -469,35 +471,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
                   reinterpret_cast<const uint4*>(own)[n * 2 + q];
           }
           __syncwarp();
-        } else {
-          const int f0 = m * 256 + (int)rank * 128 + quarter * 32;
-          if (f0 >= a.rows) continue;
-          int16_t* out = reinterpret_cast<int16_t*>(own) + lane;
-          float kept = 0.0f;
+        }
+      } else {
+        // 16 columns at a time through shared memory: two lanes a row then hold 16 neighbouring
+        // features each, so the row's largest is found in registers (a warp-wide reduction a
+        // column made this epilogue 200 cycles a column and the product 434 us, now 215 us).
+        const int f0 = m * 256 + (int)rank * 128 + quarter * 32;
+        const int n = lane >> 1, f = f0 + (lane & 1) * 16;
+        uint32_t* in = reinterpret_cast<uint32_t*>(own) + lane;
+        const uint4* back = reinterpret_cast<const uint4*>(own) + (n * kStagingPitch + (lane & 1) * 16) / 4;
+        for (int c = group * 16; c < rows && f0 < a.rows; c += 32) {
+          const int pair = c + n < rows ? a.order[row0 + c + n] : -1;
+          uint32_t r[16];
+          tmem_ld16(lanes + acc * kTileN + c, r);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const uint32_t top = __reduce_max_sync(kAll, r[i] & 0x7fffffffu);
-            const float v = __uint_as_float(r[i]), peak = __uint_as_float(top);
-            float scale;
-            if (peak >= 1e-30f && top < 0x7f800000u) {
-              scale = peak * (1.0f / 32767.0f);
-              out[i * 32] = (int16_t)__float2int_rn(v * __fdividef(32767.0f, peak));
-            } else {  // zeros, vanishing values, infinities, NaN: as bf16
-              scale = -1.0f;
-              out[i * 32] = (int16_t)BF16::round(v);
-            }
-            if (lane == i) kept = scale;
+          for (int i = 0; i < 16; ++i) in[i * kStagingPitch] = r[i];
+          __syncwarp();
+          uint32_t v[16], top = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 q = back[i];
+            v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
           }
           __syncwarp();
-          const int pair = c + lane < rows ? a.order[row0 + c + lane] : -1;
-          if (pair >= 0) a.scale[(int64_t)pair * a.blocks + f0 / kShareBlock] = kept;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {  // four lanes a row: 64 contiguous bytes
-            const int n = i * 8 + (lane >> 2), q = lane & 3;
-            const int to = __shfl_sync(kAll, pair, n);
-            if (to >= 0 && f0 + q * 8 < a.rows)
-              reinterpret_cast<uint4*>(a.share + (int64_t)to * a.rows + f0)[q] =
-                  reinterpret_cast<const uint4*>(own)[n * 4 + q];
+          for (int i = 0; i < 16; ++i) top = max(top, v[i] & 0x7fffffffu);
+          top = max(top, __shfl_xor_sync(kAll, top, 1));
+          const float peak = __uint_as_float(top);
+          const bool whole = peak >= 1e-30f && top < 0x7f800000u;
+          const float inverse = __fdividef(32767.0f, peak);
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float lo = __uint_as_float(v[2 * i]), hi = __uint_as_float(v[2 * i + 1]);
+            w[i] = __byte_perm(__float2int_rn(lo * inverse), __float2int_rn(hi * inverse), 0x5410);
+          }
+          if (!whole) {  // zeros, vanishing values, infinities, NaN: as bf16
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = BF16::round2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+          }
+          if (pair >= 0) {
+            if ((lane & 1) == 0) a.scale[(int64_t)pair * a.blocks + f0 / kShareBlock] = whole ? peak * (1.0f / 32767.0f) : -1.0f;
+            int16_t* to = a.share + (int64_t)pair * a.rows + f;
+            if (a.wide) {  // rows of whole 32-byte sectors
+              if (f < a.rows) store32(to, w);
+            } else {
+              if (f < a.rows) reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+              if (f + 8 < a.rows) reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            }
           }
           __syncwarp();
         }
@@ -518,6 +539,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
   cluster_barrier();
   tc_fence_after();
   if (warp == 1) tmem_pair_dealloc(tmem, 2 * kTileN);
+}
+
+// The rows of x in the order of the sorted pairs: one warp a row, 16 bytes a lane.
+constexpr int kSortThreads = 256;
+__global__ void __launch_bounds__(kSortThreads) expert_sort_rows(const uint16_t* __restrict__ x, int64_t x_stride,
+                                                                 int hidden, int top_k, const int32_t* __restrict__ count,
+                                                                 const int32_t* __restrict__ order,
+                                                                 uint16_t* __restrict__ sorted) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, row = blockIdx.x * (kSortThreads / 32) + (threadIdx.x >> 5);
+  if (row >= *count) return;
+  const uint4* from = reinterpret_cast<const uint4*>(x + (int64_t)(order[row] / top_k) * x_stride);
+  uint4* to = reinterpret_cast<uint4*>(sorted + (int64_t)row * hidden);
+#pragma unroll 4
+  for (int i = lane; i < hidden / 8; i += 32) to[i] = __ldg(from + i);
 }
 
 // out[token] = sum of weight * share over the token's choices, in their order; 8 features a thread.
@@ -573,9 +610,13 @@ __global__ void __launch_bounds__(kCombineThreads) expert_combine(ExpertArgs a, 
 // Up to this many pairs each pair reads its expert's weights by itself.
 constexpr int64_t kRowsPairs = 32;
 
+// From this many pairs an expert on (on the average), x is copied in sorted order first.
+constexpr int64_t kSortRows = 128;
+
 struct Sizes {
   int64_t pairs, blocks;
   bool rows;                                 // the few-pairs kernels
+  bool gather;                               // the first product gathers its rows
   int64_t order, h, share, scale, total;     // byte offsets into the workspace (offsets at 0)
 };
 bool sizes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64_t top_k, Sizes* s) {
@@ -586,6 +627,7 @@ bool sizes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64
   s->pairs = tokens * top_k;
   s->blocks = (hidden + kShareBlock - 1) / kShareBlock;
   s->rows = s->pairs <= kRowsPairs;
+  s->gather = s->pairs < kSortRows * experts;
   if (s->rows) {
     s->order = s->h = s->share = s->scale = 0;
     s->total = pad(s->pairs * inner * 4);
@@ -627,11 +669,17 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     const cuuint32_t box[5] = {kStepK, 16, 2, 4, 1};
     TTN_TRY(encode_map(name, &gate.a, bf16, 5, a.gate_up, dims, str, box));
   }
-  {  // x: one row a box, four rows a gather
+  uint16_t* sorted = (uint16_t*)(ws + s.share);  // read before the shares are written
+  if (s.gather) {  // x: one row a box, four rows a gather
     const cuuint64_t dims[2] = {hidden, (cuuint64_t)a.tokens};
     const cuuint64_t str[1] = {(cuuint64_t)a.x_stride * 2};
     const cuuint32_t box[2] = {kStepK, 1};
     TTN_TRY(encode_map(name, &gate.b, bf16, 2, a.x, dims, str, box));
+  } else {
+    const cuuint64_t dims[2] = {hidden, (cuuint64_t)s.pairs};
+    const cuuint64_t str[1] = {hidden * 2};
+    const cuuint32_t box[2] = {kStepK, 16};
+    TTN_TRY(encode_map(name, &gate.b, bf16, 2, sorted, dims, str, box));
   }
   {
     const cuuint64_t dims[3] = {inner, hidden, experts};
@@ -658,14 +706,24 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     p.m_tiles = (rows + tile - 1) / tile;
     p.blocks = (int)s.blocks;
     p.bf16 = bf16;
+    p.wide = a.hidden % 16 == 0;
     if (runs * p.m_tiles > INT32_MAX) return fail(TTN_UNSUPPORTED, "%s: more than 2^31 tiles", name);
     TTN_TRY(ensure_dynamic_smem((const void*)kernel, (int)smem));
     const int64_t pairs_of_sms = sm_count() / 2, most = runs * p.m_tiles;
     const unsigned grid = 2 * (unsigned)(most < pairs_of_sms ? most : pairs_of_sms);
     return cuda_check(launch_pdl(kernel, dim3(grid), dim3(threads), smem, stream, p, maps), name);
   };
-  TTN_TRY(products(expert_products<T, true>, gate, a.inner, a.hidden, 128, product_threads(true)));
-  TTN_TRY(products(expert_products<T, false>, down, a.hidden, a.inner, 256, product_threads(false)));
+  if (s.gather) {
+    TTN_TRY(products(expert_products<T, true, true>, gate, a.inner, a.hidden, 128, product_threads(true)));
+  } else {
+    constexpr int kRows = kSortThreads / 32;
+    TTN_TRY(cuda_check(launch_pdl(expert_sort_rows, dim3((unsigned)((s.pairs + kRows - 1) / kRows)), dim3(kSortThreads), 0,
+                                  stream, a.x, a.x_stride, a.hidden, a.top_k, (const int32_t*)(offsets + a.experts),
+                                  (const int32_t*)order, sorted),
+                       name));
+    TTN_TRY(products(expert_products<T, true, false>, gate, a.inner, a.hidden, 128, product_threads(false)));
+  }
+  TTN_TRY(products(expert_products<T, false, false>, down, a.hidden, a.inner, 256, product_threads(false)));
   const int64_t items = a.tokens * (a.hidden / 8);
   if (items + kCombineThreads > UINT32_MAX) return fail(TTN_UNSUPPORTED, "%s: output too large", name);
   return cuda_check(launch_pdl(expert_combine<T>, dim3((unsigned)((items + kCombineThreads - 1) / kCombineThreads)),
