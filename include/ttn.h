@@ -430,7 +430,7 @@ ttn_status ttn_route_experts(const ttn_tensor* logits, const float* bias, int64_
  * p = 0, log p = -inf, never among the top (left-over places: -inf and token -1); a row
  * with nothing left has log p = -inf and entropy 0.  A NaN or +inf in a row makes its
  * logprobs (of a given token), entropy and top_logprobs NaN; top_tokens then still come
- * in order, NaN first.  scale: finite, > 0.  Any of the outputs but top_* may be NULL. */
+ * in order, NaN first.  scale: 1e-6 to 1e6.  Any of the outputs but top_* may be NULL. */
 ttn_status ttn_token_logprobs(const ttn_tensor* logits, const int64_t* tokens, float scale, int64_t top,
                               float* logprobs, float* entropy, float* top_logprobs, int32_t* top_tokens,
                               ttn_stream stream);

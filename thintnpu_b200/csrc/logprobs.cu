@@ -1,21 +1,27 @@
 // Log probabilities of given tokens, entropy and the largest alternatives of vocabulary
 // rows, in one pass over the logits.
 //
-// With m the running maximum, d = scale (x - m): S = sum e^d and A = sum e^d d are kept
-// in FP32 and rescaled when m rises, so log p(x) = d - log S and the entropy is
-// log S - A / S (both terms >= 0: no cancellation).
+// With c = scale log2 e and M = c times the running maximum, rounded once, t = c x - M (one
+// fused multiply-add, so its error is |t| 2^-24 however large x is): S = sum 2^t and
+// A = sum 2^t t are kept in FP32 and rescaled by differences of M when the maximum rises.
+// log2 p(x) = t - log2 S, and the entropy is log2 S - A / S in units of log 2 (both terms
+// >= 0 but for the rounding of M: no cancellation).
 //
-// The alternatives ride along.  A warp reads 32 16-byte vectors (a segment: 256 16-bit
-// logits) at a time and needs their maximum for m anyway; it leaves that maximum in
-// shared memory.  The n largest logits of a row lie in the n segments with the largest
-// maxima (in the order value, then segment: an element elsewhere has n segment maxima
-// ahead of it), so afterwards only those n segments are read again (they are in L2) and
-// only their elements that come no later than the n-th segment maximum are compared.
+// The alternatives ride along.  A warp reads segments of 64 16-byte vectors (512 16-bit
+// logits) and needs their maxima for M anyway; it leaves them in shared memory.  The n-th
+// largest of 32 lanes' maxima over those is a floor: n elements are at least that large, so
+// the n largest of the row lie in the segments whose maximum reaches it.  Only those (about
+// 30 of 250 for n = 20) are read again (they are in L2), and their elements from the floor
+// up, usually n to 2n, are put in order by counting the larger ones.
+//
+// Where the maximum's magnitude is 2^100 or more, c x would overflow; c is 2^-60 there.
+// Values that differ at all then differ by 2^77 or more, so all but those equal to the
+// maximum vanish with it as they do with any allowed scale (>= 1e-6), and M is exact.
 //
 // A row is read by a cluster of 1 to 8 CTAs, one slice each; CTA 0 joins their (m, S, A)
 // and their sorted lists through distributed shared memory.
 //
-// Bound: the row's bytes; the arithmetic (about 6 instructions and one exp2 a logit) has
+// Bound: the row's bytes; the arithmetic (about 8 instructions and one exp2 a logit) has
 // to stay below the 11 issue slots a 16-bit logit at copy speed.
 #include <cooperative_groups.h>
 
@@ -31,7 +37,10 @@ namespace cg = cooperative_groups;
 constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32;
-constexpr int kLpUnroll = 4;  // vectors in flight a thread
+constexpr int kLpGroup = 2;     // vectors of a lane in a segment
+constexpr int kLpUnroll = 2;    // segments in flight a warp
+constexpr int kLpMaxRanks = 8;  // CTAs of a row
+constexpr int kLpHeld = 512;    // candidates of a CTA (>= 32 a warp)
 constexpr int64_t kLpMaxVocabulary = 1 << 20;
 constexpr uint32_t kAll = 0xffffffffu;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
@@ -54,60 +63,84 @@ __device__ __forceinline__ uint64_t entry(uint32_t key, uint32_t place) {
   return key ? (uint64_t)key << 32 | (uint32_t)~place : 0ull;
 }
 
-// Sorts one entry a lane, largest first (bitonic).
-__device__ __forceinline__ uint64_t sort32(uint64_t v, int lane) {
+// The largest value of the warp, NaN if there is one.
+__device__ __forceinline__ float warp_largest(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Sorts one key or entry a lane, largest first (bitonic).  Not inlined, as merge32: code that
+// runs at most once a row should not be long.
+template <typename K>
+__device__ __noinline__ K sort32(K v, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
     for (int d = size >> 1; d; d >>= 1) {
-      const uint64_t o = __shfl_xor_sync(kAll, v, d);
+      const K o = __shfl_xor_sync(kAll, v, d);
       const bool larger = ((lane & d) == 0) == ((lane & size) == 0 || size == 32);
       v = larger ? max(v, o) : min(v, o);
     }
   return v;
 }
 // The 32 largest of two sorted lists, sorted: `other` reversed against `list`, then a bitonic merge.
-__device__ __forceinline__ uint64_t merge32(uint64_t list, uint64_t other, int lane) {
-  uint64_t v = max(list, __shfl_sync(kAll, other, 31 - lane));
+template <typename K>
+__device__ __noinline__ K merge32(K list, K other, int lane) {
+  K v = max(list, __shfl_sync(kAll, other, 31 - lane));
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
-    const uint64_t o = __shfl_xor_sync(kAll, v, d);
+    const K o = __shfl_xor_sync(kAll, v, d);
     v = (lane & d) == 0 ? max(v, o) : min(v, o);
   }
   return v;
 }
-
 struct LpPart {  // what a warp or a CTA knows of its part of the row
-  float m, s, a;
+  float m, s, a;     // M, S, A
   uint32_t top_key;  // key of the largest logit
 };
+// The factor of logits whose maximum is `most`.
+__device__ __forceinline__ float factor(float most, float c) {
+  return fabsf(most) < 1.2676506e30f ? c : 8.6736174e-19f;  // 2^100, 2^-60
+}
 // b joined to a: both rescaled to the larger maximum.  A part without live logits has s = 0.
 __device__ __forceinline__ LpPart join(const LpPart& a, const LpPart& b, float c) {
   LpPart r;
   r.top_key = max(a.top_key, b.top_key);
-  if (b.s == 0.0f || a.s == 0.0f) {
-    const LpPart& o = b.s == 0.0f ? a : b;
+  if (b.s == 0.0f || a.s == 0.0f || factor(key_value(a.top_key), c) != factor(key_value(b.top_key), c)) {
+    // one has nothing, or nothing beside the other
+    const LpPart& o = b.s == 0.0f || (a.s != 0.0f && a.top_key > b.top_key) ? a : b;
     r.m = o.m, r.s = o.s, r.a = o.a;
     return r;
   }
   r.m = fmaxf(a.m, b.m);
-  const float ta = fmaxf((a.m - r.m) * c, -256.0f), tb = fmaxf((b.m - r.m) * c, -256.0f);
+  const float ta = fmaxf(a.m - r.m, -256.0f), tb = fmaxf(b.m - r.m, -256.0f);
   const float fa = exp2f(ta), fb = exp2f(tb);
   r.s = a.s * fa + b.s * fb;
   r.a = (a.a + a.s * ta) * fa + (b.a + b.s * tb) * fb;
   return r;
 }
 
+// Joins the parts of the first `count` lanes (a power of two), pairwise; lane 0 has the whole.
+__device__ __forceinline__ LpPart join_lanes(LpPart p, int count, float c) {
+  for (int d = 1; d < count; d <<= 1) {
+    const LpPart o = {__shfl_xor_sync(kAll, p.m, d), __shfl_xor_sync(kAll, p.s, d), __shfl_xor_sync(kAll, p.a, d),
+                      __shfl_xor_sync(kAll, p.top_key, d)};
+    p = join(p, o, c);
+  }
+  return p;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs(LpArgs a) {
-  extern __shared__ uint32_t seg_key[];  // [segments of the slice], only with a.top
-  __shared__ uint64_t lists[kLpWarps][32];
-  __shared__ uint64_t buffer[kLpWarps][64];
+__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs(LpArgs a) {
+  extern __shared__ float seg_top[];  // largest logit of each segment of the slice, only with a.top
+  __shared__ uint64_t buffer[kLpHeld];
+  __shared__ int held;
   __shared__ LpPart parts[kLpWarps];
   __shared__ LpPart cta_part;
   __shared__ uint64_t cta_list[32];
   constexpr int kVec = T::kVec;
-  constexpr int kSeg = 32 * kVec;
+  constexpr int kSeg = kLpGroup * 32 * kVec;
   using raw = typename T::raw;
   const cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -120,62 +153,129 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs(LpArgs a) {
   const int segments = (length + kSeg - 1) / kSeg;
   const int seg0 = rank * a.slice, seg1 = min(segments, seg0 + a.slice);
   const float c = a.scale * kLog2e;
-
-  // One vector of a lane: whole where it lies inside the row, else element by element
-  // with -inf outside.
-  auto load = [&](int seg) {
-    const int at = seg * kSeg + lane * kVec - shift;
-    uint4 v;
-    if (at >= 0 && at + kVec <= a.vocabulary) {
-      v = __ldg(reinterpret_cast<const uint4*>(base + at));
-    } else {
-      constexpr raw kNone = sizeof(raw) == 4 ? (raw)0xff800000u : std::is_same<T, F16>::value ? (raw)0xfc00u : (raw)0xff80u;
-      __align__(16) raw e[kVec];
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) e[i] = at + i >= 0 && at + i < a.vocabulary ? base[at + i] : kNone;
-      v = *reinterpret_cast<uint4*>(e);
-    }
-    return v;
-  };
-
-  LpPart p = {0.0f, 0.0f, 0.0f, 0u};  // m: the warp's; s, a: this lane's
-  bool started = false;
-  for (int seg = seg0 + warp; seg < seg1; seg += kLpWarps * kLpUnroll) {
-    uint4 v[kLpUnroll];
-#pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u)
-      if (seg + u * kLpWarps < seg1) v[u] = load(seg + u * kLpWarps);
-#pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u) {
-      if (seg + u * kLpWarps >= seg1) break;
-      float f[kVec];
-      T::unpack(v[u], f);
-      uint32_t k = 0;
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) k = max(k, order_key(f[i]));
-      k = __reduce_max_sync(kAll, k);
-      if (a.top && lane == 0) seg_key[seg + u * kLpWarps - seg0] = k;
-      if (!k) continue;  // nothing but masked logits
-      p.top_key = max(p.top_key, k);
-      const float sm = key_value(k);
-      if (!started || sm > p.m) {  // the same in all lanes
-        if (started) {
-          const float t = fmaxf((p.m - sm) * c, -256.0f), scale = exp2f(t);
-          p.a = (p.a + p.s * t) * scale;
-          p.s *= scale;
-        }
-        p.m = sm;
-        started = true;
-      }
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        const float t = fmaxf((f[i] - p.m) * c, -256.0f);  // masked logits: e = 0 and t finite
-        const float e = ex2_approx(t);
-        p.s += e;
-        p.a = fmaf(e, t, p.a);
-      }
+  float given = 0.0f;  // thread 0 of CTA 0: the given token's logit
+  bool has_given = false;
+  if (threadIdx.x == 0) {
+    held = 0;
+    if (rank == 0 && a.logprobs) {
+      const int64_t token = a.tokens[row];
+      has_given = token >= 0 && token < a.vocabulary;
+      if (has_given) given = T::get(base[token]);
     }
   }
+
+  // One vector of a lane; where a segment does not lie wholly inside the row, element by
+  // element with -inf outside.
+  auto whole = [&](int seg) { return seg * kSeg >= shift && (seg + 1) * kSeg <= length; };
+  auto load = [&](int seg, int g, bool inside) {
+    const int at = seg * kSeg + (g * 32 + lane) * kVec - shift;
+    if (inside) return __ldg(reinterpret_cast<const uint4*>(base + at));
+    constexpr raw kNone = sizeof(raw) == 4 ? (raw)0xff800000u : std::is_same<T, F16>::value ? (raw)0xfc00u : (raw)0xff80u;
+    __align__(16) raw e[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) e[i] = at + i >= 0 && at + i < a.vocabulary ? base[at + i] : kNone;
+    return *reinterpret_cast<uint4*>(e);
+  };
+
+  // the maximum and M are the warp's, S and A this lane's, in two halves (packed arithmetic)
+  const float ninf = -__int_as_float(0x7f800000);
+  float most = ninf;
+  bool bad = false;  // a NaN or +inf
+  float by = c;
+  float m = 0.0f;
+  unsigned long long s2 = 0, a2 = 0;
+  auto add = [&](int seg, const uint4 (&v)[kLpUnroll][kLpGroup], int count) {
+    float top[kLpUnroll], rise = ninf;
+#pragma unroll
+    for (int u = 0; u < kLpUnroll; ++u) {
+      if (u >= count) break;
+      float l = T::largest(v[u][0]);
+#pragma unroll
+      for (int g = 1; g < kLpGroup; ++g) l = max_nan(l, T::largest(v[u][g]));
+      top[u] = warp_largest(l);
+      rise = max_nan(rise, top[u]);
+      if (a.top && lane == 0) seg_top[seg + u * kLpWarps - seg0] = top[u];
+    }
+    if (!(rise <= most)) {  // the same in all lanes
+      if (rise < __int_as_float(0x7f800000)) {
+        const float last = by;
+        by = factor(rise, c);
+        const float next = rise * by;
+        if (most != ninf) {
+          const float t = last == by ? fmaxf(m - next, -256.0f) : -256.0f, shrink = exp2f(t);
+          a2 = f2_mul(f2_fma(s2, f2_pack(t, t), a2), f2_pack(shrink, shrink));
+          s2 = f2_mul(s2, f2_pack(shrink, shrink));
+        }
+        m = next;
+        most = rise;
+      } else {
+        bad = true;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kLpUnroll; ++u) {
+      if (u >= count) break;
+      if (top[u] == ninf) continue;  // nothing but masked logits
+#pragma unroll
+      for (int g = 0; g < kLpGroup; ++g) {
+        float f[kVec];
+        T::unpack(v[u][g], f);
+#pragma unroll
+        for (int i = 0; i < kVec; i += 2) {
+          const float2 d = f2_unpack(f2_fma(f2_pack(f[i], f[i + 1]), f2_pack(by, by), f2_pack(-m, -m)));
+          const float t0 = fmaxf(d.x, -256.0f), t1 = fmaxf(d.y, -256.0f);  // masked logits: 2^t = 0 and t finite
+          const unsigned long long e = f2_pack(ex2_approx(t0), ex2_approx(t1));
+          s2 = f2_add(s2, e);
+          a2 = f2_fma(e, f2_pack(t0, t1), a2);
+        }
+      }
+    }
+  };
+  int seg = seg0 + warp;
+  uint4 v[kLpUnroll][kLpGroup];
+  // batches wholly inside the row (all but the row's ends), then the rest segment by segment
+  if (seg < seg1 && !whole(seg)) {
+#pragma unroll
+    for (int g = 0; g < kLpGroup; ++g) v[0][g] = load(seg, g, false);
+    add(seg, v, 1);
+    seg += kLpWarps;
+  }
+  constexpr int kBatch = kLpWarps * kLpUnroll;
+  auto fits = [&](int first) {
+    const int last = first + kLpWarps * (kLpUnroll - 1);
+    return last < seg1 && whole(last);
+  };
+  auto fetch = [&](int first, uint4 (&to)[kLpUnroll][kLpGroup]) {
+#pragma unroll
+    for (int u = 0; u < kLpUnroll; ++u)
+#pragma unroll
+      for (int g = 0; g < kLpGroup; ++g) to[u][g] = load(first + u * kLpWarps, g, true);
+  };
+  if (fits(seg)) {  // the next batch's loads are in flight while one is added up
+    uint4 next[kLpUnroll][kLpGroup];
+    fetch(seg, v);
+    while (true) {
+      const bool more = fits(seg + kBatch);
+      if (more) fetch(seg + kBatch, next);
+      add(seg, v, kLpUnroll);
+      seg += kBatch;
+      if (!more) break;
+      const bool again = fits(seg + kBatch);
+      if (again) fetch(seg + kBatch, v);
+      add(seg, next, kLpUnroll);
+      seg += kBatch;
+      if (!again) break;
+    }
+  }
+#pragma unroll 1
+  for (; seg < seg1; seg += kLpWarps) {
+    const bool inside = whole(seg);
+#pragma unroll
+    for (int g = 0; g < kLpGroup; ++g) v[0][g] = load(seg, g, inside);
+    add(seg, v, 1);
+  }
+  const float2 s_halves = f2_unpack(s2), a_halves = f2_unpack(a2);
+  LpPart p = {m, s_halves.x + s_halves.y, a_halves.x + a_halves.y, bad ? kAll : order_key(most)};
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
     p.s += __shfl_xor_sync(kAll, p.s, d);
@@ -183,92 +283,122 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs(LpArgs a) {
   }
   if (lane == 0) parts[warp] = p;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    LpPart all = parts[0];
-    for (int i = 1; i < kLpWarps; ++i) all = join(all, parts[i], c);
-    cta_part = all;
+  if (warp == 0) {
+    const LpPart all = join_lanes(parts[lane % kLpWarps], kLpWarps, c);
+    if (lane == 0) cta_part = all;
   }
 
   if (a.top) {
-    // sorted lists of the largest entries: one a warp, joined pairwise
-    auto join_lists = [&](uint64_t list) {
-      lists[warp][lane] = list;
-      for (int half = kLpWarps / 2; half; half >>= 1) {
-        __syncthreads();
-        if (warp < half) {
-          list = merge32(list, lists[warp + half][lane], lane);
-          lists[warp][lane] = list;
+    const int count = max(seg1 - seg0, 0), own = (count - warp + kLpWarps - 1) / kLpWarps;
+    // floor: the n-th largest of the lanes' maxima over the segment maxima (n <= 32)
+    uint32_t key = 0;
+    for (int i = lane; i < count; i += 32) key = max(key, order_key(seg_top[i]));
+    const uint32_t floor_key = __shfl_sync(kAll, sort32(key, lane), a.top - 1);
+    const float floor_value = key_value(floor_key);  // -inf: fewer live segments than that
+    // First the elements from the floor up are gathered in no particular order, and each one's
+    // place is the number of larger ones.  Where they are too many for that (many equal or
+    // rising logits), a second time into sorted lists, one a warp: once a list is full only what
+    // beats its n-th entry gets in.
+    uint64_t list = 0, last = 0;
+    for (bool sorted = false;; sorted = true) {
+      for (int i0 = 0; i0 < own; i0 += 32) {
+        const int i = i0 + lane;
+        uint32_t open = __ballot_sync(kAll, i < own && !(seg_top[min(i, own - 1) * kLpWarps + warp] < floor_value));
+        while (open) {  // two segments' loads in flight
+          const int s0 = seg0 + (i0 + __ffs(open) - 1) * kLpWarps + warp;
+          open &= open - 1;
+          const int s1 = open ? seg0 + (i0 + __ffs(open) - 1) * kLpWarps + warp : s0;
+          const bool two = open != 0;
+          open &= open - 1;
+          uint4 v[2][kLpGroup];
+#pragma unroll
+          for (int g = 0; g < kLpGroup; ++g) {
+            v[0][g] = load(s0, g, whole(s0));
+            v[1][g] = load(s1, g, whole(s1));
+          }
+          uint32_t reach = 0;  // bit (u * kLpGroup + g) * kVec + q
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int g = 0; g < kLpGroup; ++g) {
+              float f[kVec];
+              T::unpack(v[u][g], f);
+#pragma unroll
+              for (int q = 0; q < kVec; ++q)
+                reach |= (uint32_t)(!(f[q] < floor_value)) << ((u * kLpGroup + g) * kVec + q);
+            }
+          if (!two) reach &= (1u << (kLpGroup * kVec)) - 1;
+          while (__any_sync(kAll, reach)) {  // few: each element is read once more by itself
+            uint64_t e = 0;
+            if (reach) {
+              const int bit = __ffs(reach) - 1, g = bit / kVec;
+              reach &= reach - 1;
+              const int place = (g < kLpGroup ? s0 : s1) * kSeg + ((g % kLpGroup) * 32 + lane) * kVec + bit % kVec - shift;
+              if (place >= 0 && place < a.vocabulary) e = entry(order_key(T::get(base[place])), place);
+            }
+            if (!sorted) {
+              const uint32_t vote = __ballot_sync(kAll, e != 0);
+              int at = 0;
+              if (lane == 0) at = atomicAdd(&held, __popc(vote));
+              at = __shfl_sync(kAll, at, 0) + __popc(vote & ((1u << lane) - 1));
+              if (e && at < kLpHeld) buffer[at] = e;
+            } else if (__any_sync(kAll, e > last)) {
+              list = merge32(list, sort32(e > last ? e : (uint64_t)0, lane), lane);
+              last = __shfl_sync(kAll, list, a.top - 1);
+            }
+          }
         }
       }
       __syncthreads();
-      return lists[0][lane];
-    };
-    const int count = max(seg1 - seg0, 0);
-    uint64_t list = 0;
-    for (int i = warp * 32; i < count; i += kLpThreads) {
-      const uint64_t mine = i + lane < count ? entry(seg_key[i + lane], i + lane) : 0ull;
-      if (__any_sync(kAll, mine > __shfl_sync(kAll, list, 31))) list = merge32(list, sort32(mine, lane), lane);
+      if (sorted || held <= kLpHeld) break;
     }
-    const uint64_t best = join_lists(list);
-    // the n-th largest segment maximum: no element behind it is among the n largest
-    const uint32_t floor_key = (uint32_t)(__shfl_sync(kAll, best, a.top - 1) >> 32);
-    list = 0;
-    int held = 0;
-    uint64_t* mine = buffer[warp];
-    __syncthreads();  // lists[0] is read
-    for (int j = warp; j < a.top; j += kLpWarps) {
-      const uint64_t chosen = __shfl_sync(kAll, best, j);
-      if (!chosen) break;
-      const int seg = seg0 + (int)~(uint32_t)chosen;
-      const uint4 v = load(seg);
-      float f[kVec];
-      T::unpack(v, f);
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        const uint32_t k = order_key(f[i]);
-        const bool in = k && k >= floor_key;
-        const uint32_t vote = __ballot_sync(kAll, in);
-        if (!vote) continue;
-        if (in) mine[held + __popc(vote & ((1u << lane) - 1))] = entry(k, seg * kSeg + lane * kVec + i - shift);
-        held += __popc(vote);
-        __syncwarp();
-        if (held >= 32) {
-          list = merge32(list, sort32(mine[lane], lane), lane);
-          __syncwarp();
-          const uint64_t rest = mine[32 + lane];
-          __syncwarp();
-          mine[lane] = rest;
-          held -= 32;
-          __syncwarp();
+    if (held <= kLpHeld) {
+      for (int i = threadIdx.x; i < max(held, 32); i += kLpThreads) {
+        const uint64_t e = i < held ? buffer[i] : 0ull;
+        int place = i < held ? 0 : i;  // places that no entry takes hold none
+#pragma unroll 4
+        for (int j = 0; j < held; ++j) place += i < held && buffer[j] > e;
+        if (place < 32) cta_list[place] = e;
+      }
+    } else {
+      buffer[warp * 32 + lane] = list;
+      for (int half = kLpWarps / 2; half; half >>= 1) {
+        __syncthreads();
+        if (warp < half) {
+          list = merge32(list, buffer[(warp + half) * 32 + lane], lane);
+          buffer[warp * 32 + lane] = list;
         }
       }
+      if (warp == 0) cta_list[lane] = list;
     }
-    if (held) list = merge32(list, sort32(lane < held ? mine[lane] : 0ull, lane), lane);
-    list = join_lists(list);
-    if (warp == 0) cta_list[lane] = list;
   }
   if (ranks > 1)
     cluster.sync();
   else
     __syncthreads();
   if (rank == 0 && warp == 0) {
-    LpPart all = cta_part;
-    uint64_t list = a.top ? cta_list[lane] : 0ull;
-    for (int r = 1; r < ranks; ++r) {
-      all = join(all, *cluster.map_shared_rank(&cta_part, r), c);
-      if (a.top) list = merge32(list, cluster.map_shared_rank(cta_list, r)[lane], lane);
-    }
-    const float nan = __int_as_float(0x7fffffff), ninf = -__int_as_float(0x7f800000);
+    uint64_t lists_of[kLpMaxRanks];
+#pragma unroll
+    for (int r = 0; r < kLpMaxRanks; ++r)  // all remote reads in flight together
+      lists_of[r] = a.top && r < ranks ? cluster.map_shared_rank(cta_list, r)[lane] : 0ull;
+    const LpPart all = join_lanes(*cluster.map_shared_rank(&cta_part, lane & (ranks - 1)), ranks, c);
+#pragma unroll
+    for (int half = kLpMaxRanks / 2; half; half >>= 1)
+      if (half < ranks) {
+#pragma unroll
+        for (int r = 0; r < half; ++r) lists_of[r] = merge32(lists_of[r], lists_of[r + half], lane);
+      }
+    const uint64_t list = lists_of[0];
+    const float nan = __int_as_float(0x7fffffff);
     const bool bad = all.top_key >= 0xff800000u;  // +inf or NaN
     const bool empty = all.top_key == 0u;
-    const float log_total = logf(all.s);
-    auto logp = [&](float x) { return bad ? nan : empty || x == ninf ? ninf : (x - all.m) * a.scale - log_total; };
+    const float log_total = log2f(all.s);
+    // log p(m) = log 2 ((c m - M) - log2 S), of which c m - M is what M's rounding left
+    const float m = key_value(all.top_key), log_p_m = (fmaf(m, factor(m, c), -all.m) - log_total) * kLn2;
+    auto logp = [&](float x) { return bad ? nan : empty || x == ninf ? ninf : fmaf(x - m, a.scale, log_p_m); };
     if (lane == 0) {
-      if (a.logprobs) {
-        const int64_t token = a.tokens[row];
-        a.logprobs[row] = token >= 0 && token < a.vocabulary ? logp(T::get(base[token])) : 0.0f;
-      }
-      if (a.entropy) a.entropy[row] = bad ? nan : empty ? 0.0f : log_total - all.a / all.s * kLn2;
+      if (a.logprobs) a.logprobs[row] = has_given ? logp(given) : 0.0f;
+      if (a.entropy) a.entropy[row] = bad ? nan : empty ? 0.0f : (log_total - all.a / all.s) * kLn2;
     }
     if (lane < a.top) {
       const uint32_t k = (uint32_t)(list >> 32);
@@ -281,11 +411,11 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs(LpArgs a) {
 
 template <typename T>
 ttn_status launch_logprobs(const char* name, LpArgs a, cudaStream_t stream) {
-  constexpr int kSeg = 32 * T::kVec;
+  constexpr int kSeg = kLpGroup * 32 * T::kVec;
   const int segments = (int)((a.vocabulary + T::kVec - 1 + kSeg - 1) / kSeg);  // at the largest shift
   // Few rows: split each over a cluster, as long as a CTA keeps two rounds of its warps.
   int ranks = 1;
-  while (ranks < 8 && a.rows * ranks * 2 <= 2 * sm_count() && segments > ranks * kLpWarps * kLpUnroll) ranks *= 2;
+  while (ranks < kLpMaxRanks && a.rows * ranks * 2 <= 2 * sm_count() && segments > ranks * kLpWarps * kLpUnroll) ranks *= 2;
   a.slice = (segments + ranks - 1) / ranks;
   const size_t smem = a.top ? (size_t)a.slice * 4 : 0;
   cudaLaunchConfig_t config = {};
@@ -318,7 +448,7 @@ extern "C" ttn_status ttn_token_logprobs(const ttn_tensor* logits, const int64_t
   if (v > 1 && logits->strides[1] != 1) return fail(TTN_UNSUPPORTED, "%s: the last stride must be 1", name);
   if (top < 0 || top > kLpMaxTop || top > v)
     return fail(TTN_UNSUPPORTED, "%s: top %lld outside [0, min(%d, vocabulary)]", name, (long long)top, kLpMaxTop);
-  if (!(scale > 0.0f) || scale > 1e30f) return fail(TTN_INVALID_ARG, "%s: scale must be positive and finite", name);
+  if (!(scale >= 1e-6f && scale <= 1e6f)) return fail(TTN_INVALID_ARG, "%s: scale must be in [1e-6, 1e6]", name);
   if (rows > INT32_MAX / 8) return fail(TTN_UNSUPPORTED, "%s: too many rows", name);
   if (rows == 0) return TTN_OK;
   if (top && (!top_logprobs || !top_tokens)) return fail(TTN_INVALID_ARG, "%s: null top output", name);

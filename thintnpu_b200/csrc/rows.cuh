@@ -8,8 +8,19 @@
 
 namespace ttn {
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 struct F32 {
   using raw = uint32_t;
+  // the largest of a vector's elements, NaN if one is
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)),
+                   max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
   static constexpr int kVec = 4;  // elements in 16 bytes
   static __device__ __forceinline__ float get(raw b) { return __uint_as_float(b); }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
@@ -20,6 +31,11 @@ struct F16 {
   using raw = uint16_t;
   static constexpr int kVec = 8;
   static __device__ __forceinline__ float get(raw b) { return __half2float(__ushort_as_half(b)); }
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const float2 f = __half22float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    return max_nan(f.x, f.y);
+  }
   static __device__ __forceinline__ float2 two(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
   static __device__ __forceinline__ uint32_t round2(float lo, float hi) {
     __half2 h = __floats2half2_rn(lo, hi);
@@ -39,6 +55,11 @@ struct BF16 {
   using raw = uint16_t;
   static constexpr int kVec = 8;
   static __device__ __forceinline__ float get(raw b) { return __uint_as_float((uint32_t)b << 16); }
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const float2 f = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    return max_nan(f.x, f.y);
+  }
   static __device__ __forceinline__ float2 two(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }

@@ -613,28 +613,39 @@ _ROW_DTYPES = {torch.float16: _lib.F16, torch.float32: _lib.F32, torch.bfloat16:
 def _call_on(device: torch.device, function: str, *args) -> None:
     """``call`` with the current stream of the tensors' device, which becomes the current
     device for the launch where it is another one."""
-    if device.index == torch.cuda.current_device():
-        call(function, *args, torch.cuda.current_stream().cuda_stream)
-        return
-    with torch.cuda.device(device):
-        call(function, *args, torch.cuda.current_stream().cuda_stream)
+    index = device.index
+    status_of = getattr(_lib.lib(), function)
+    if index == torch._C._cuda_getDevice():
+        status = status_of(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = status_of(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(function, status)
+
+
+def _inputs(what: str, *tensors) -> None:
+    """``_cuda`` of each; the common case without building its messages."""
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.requires_grad:
+            _cuda(t, what)
 
 
 def _score_rows(x: torch.Tensor, what: str) -> TtnTensor:
     """Descriptor of a [rows, columns] view of f16, bf16 or f32 scores."""
-    _cuda(x, what)
-    _require(x.dim() == 2, f"{what}: logits must be [rows, columns]")
+    _inputs(what, x)
     dtype = _ROW_DTYPES.get(x.dtype)
-    _require(dtype is not None, f"{what}: unsupported dtype {x.dtype}: float16/bfloat16/float32 only")
-    d = TtnTensor(x.data_ptr(), 2, dtype)
-    d.sizes[0], d.sizes[1] = x.shape
-    d.strides[0], d.strides[1] = x.stride()
-    return d
+    if x.dim() != 2:
+        _fail(f"{what}: logits must be [rows, columns]")
+    if dtype is None:
+        _fail(f"{what}: unsupported dtype {x.dtype}: float16/bfloat16/float32 only")
+    return TtnTensor(x.data_ptr(), 2, dtype, tuple(x.shape), x.stride())
 
 
 def _like_output(t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device, what: str) -> None:
-    _require(isinstance(t, torch.Tensor) and tuple(t.shape) == shape and t.dtype == dtype and t.device == device
-             and t.is_contiguous(), f"{what} must be contiguous {dtype} {list(shape)} on {device}")
+    if not (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype == dtype and t.device == device
+            and t.is_contiguous()):
+        _fail(f"{what} must be contiguous {dtype} {list(shape)} on {device}")
 
 
 def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: Optional[torch.Tensor] = None,
@@ -653,23 +664,25 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     pair to fill."""
     what = "route_experts"
     d = _score_rows(logits, what)
-    _require(score in ("softmax", "sigmoid"), f"{what}: score must be 'softmax' or 'sigmoid'")
+    if score not in ("softmax", "sigmoid"):
+        _fail(f"{what}: score must be 'softmax' or 'sigmoid'")
     rows, experts = logits.shape
     device = logits.device
     bias_ptr = None
     if bias is not None:
-        _cuda(bias, what)
-        _like_output(bias, (experts,), torch.float32, device, f"{what}: bias")
+        _inputs(what, bias)
+        _like_output(bias, (experts,), torch.float32, device, "route_experts: bias")
         bias_ptr = bias.data_ptr()
     top_k = int(top_k)
-    _require(1 <= top_k <= experts, f"{what}: top_k must be in [1, experts]")
+    if not 1 <= top_k <= experts:
+        _fail(f"{what}: top_k must be in [1, experts]")
     if out is None:
         weights = torch.empty((rows, top_k), dtype=torch.float32, device=device)
         ids = torch.empty((rows, top_k), dtype=torch.int32, device=device)
     else:
         weights, ids = out
-        _like_output(weights, (rows, top_k), torch.float32, device, f"{what}: out weights")
-        _like_output(ids, (rows, top_k), torch.int32, device, f"{what}: out experts")
+        _like_output(weights, (rows, top_k), torch.float32, device, "route_experts: out weights")
+        _like_output(ids, (rows, top_k), torch.int32, device, "route_experts: out experts")
     flags = (_lib.ROUTE_SIGMOID if score == "sigmoid" else 0) | (_lib.ROUTE_RENORMALIZE if renormalize else 0)
     _call_on(device, "ttn_route_experts", _ref(d), bias_ptr, top_k, groups,
              groups if top_groups is None else top_groups, group_top, flags, scale, weights.data_ptr(),
@@ -697,33 +710,34 @@ def expert_mlp(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, ga
     stay FP32), so they have to lie in its range.  ``workspace``: at least
     ``expert_mlp_workspace_size`` bytes of uint8, 256-byte aligned, for one call at a time."""
     what = "expert_mlp"
-    for t in (x, experts, weights, gate_up, down):
-        _cuda(t, what)
+    _inputs(what, x, experts, weights, gate_up, down)
     device, dtype = x.device, x.dtype
-    _require(dtype == torch.float16 or dtype == torch.bfloat16, f"{what} supports float16/bfloat16")
-    _require(x.dim() == 2 and (x.stride(1) == 1 or x.size(1) == 1), f"{what}: x must be [tokens, hidden] with unit-stride rows")
+    if dtype != torch.float16 and dtype != torch.bfloat16:
+        _fail(f"{what} supports float16/bfloat16")
+    if x.dim() != 2 or (x.stride(1) != 1 and x.size(1) != 1):
+        _fail(f"{what}: x must be [tokens, hidden] with unit-stride rows")
     tokens, hidden = x.shape
-    _require(gate_up.dim() == 3 and gate_up.size(1) % 2 == 0 and gate_up.size(2) == hidden,
-             f"{what}: gate_up must be [experts, 2*inner, hidden]")
+    if gate_up.dim() != 3 or gate_up.size(1) % 2 or gate_up.size(2) != hidden:
+        _fail(f"{what}: gate_up must be [experts, 2*inner, hidden]")
     num, inner = gate_up.size(0), gate_up.size(1) // 2
-    _require(gate_up.dtype == dtype and gate_up.device == device and gate_up.is_contiguous(),
-             f"{what}: gate_up must be contiguous, of x's dtype and device")
-    _like_output(down, (num, hidden, inner), dtype, device, f"{what}: down")
-    _require(experts.dim() == 2 and experts.size(0) == tokens, f"{what}: experts must be [tokens, top_k]")
+    if gate_up.dtype != dtype or gate_up.device != device or not gate_up.is_contiguous():
+        _fail(f"{what}: gate_up must be contiguous, of x's dtype and device")
+    _like_output(down, (num, hidden, inner), dtype, device, "expert_mlp: down")
+    if experts.dim() != 2 or experts.size(0) != tokens:
+        _fail(f"{what}: experts must be [tokens, top_k]")
     top_k = experts.size(1)
-    _like_output(experts, (tokens, top_k), torch.int32, device, f"{what}: experts")
-    _like_output(weights, (tokens, top_k), torch.float32, device, f"{what}: weights")
+    _like_output(experts, (tokens, top_k), torch.int32, device, "expert_mlp: experts")
+    _like_output(weights, (tokens, top_k), torch.float32, device, "expert_mlp: weights")
     if out is None:
         out = torch.empty((tokens, hidden), dtype=dtype, device=device)
-    else:
-        _require(out.shape == x.shape and out.dtype == dtype and out.device == device
-                 and (out.stride(1) == 1 or hidden == 1), f"{what}: out must match x, with unit-stride rows")
-    need = expert_mlp_workspace_size(tokens, hidden, inner, num, top_k)
+    elif not (out.shape == x.shape and out.dtype == dtype and out.device == device
+              and (out.stride(1) == 1 or hidden == 1)):
+        _fail(f"{what}: out must match x, with unit-stride rows")
     if workspace is None:
+        need = expert_mlp_workspace_size(tokens, hidden, inner, num, top_k)
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    else:
-        _require(workspace.dtype == torch.uint8 and workspace.device == device and workspace.is_contiguous(),
-                 f"{what}: workspace must be contiguous uint8 on x's device")
+    elif not (workspace.dtype == torch.uint8 and workspace.device == device and workspace.is_contiguous()):
+        _fail(f"{what}: workspace must be contiguous uint8 on x's device")
     _call_on(device, "ttn_expert_mlp", _ROW_DTYPES[dtype], x.data_ptr(), x.stride(0), tokens, hidden,
              experts.data_ptr(), weights.data_ptr(), top_k, gate_up.data_ptr(), down.data_ptr(), num, inner,
              out.data_ptr(), out.stride(0), workspace.data_ptr(), workspace.numel())
@@ -743,7 +757,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     float32 and (the last) int32.
 
     logits: [rows, vocabulary] f16, bf16 or f32, unit last stride, any row stride, at most
-    2^20 columns; tokens: int64 [rows].  A token outside the vocabulary marks a row
+    2^20 columns; tokens: int64 [rows]; scale: 1e-6 to 1e6.  A token outside the vocabulary marks a row
     without a given token: its log probability is 0.  The ``top`` (at most 32) largest
     come in falling order, ties to the lower index.  Logits of -inf are masked: never
     among the top (left-over places hold -inf and token -1), log probability -inf; a row
@@ -752,12 +766,13 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     what = "token_logprobs"
     d = _score_rows(logits, what)
     rows, device = logits.size(0), logits.device
-    _cuda(tokens, what)
-    _like_output(tokens, (rows,), torch.int64, device, f"{what}: tokens")
+    _inputs(what, tokens)
+    _like_output(tokens, (rows,), torch.int64, device, "token_logprobs: tokens")
     top = int(top)
+    if not 0 <= top <= logits.size(1):
+        _fail(f"{what}: top must be in [0, vocabulary]")
     logprobs = torch.empty(rows, dtype=torch.float32, device=device)
     entropy = torch.empty(rows, dtype=torch.float32, device=device)
-    _require(0 <= top <= logits.size(1), f"{what}: top must be in [0, vocabulary]")
     top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
     top_tokens = torch.empty((rows, top), dtype=torch.int32, device=device)
     _call_on(device, "ttn_token_logprobs", _ref(d), tokens.data_ptr(), scale, top, logprobs.data_ptr(),
