@@ -38,7 +38,7 @@ constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32;
 constexpr int kLpGroup = 2;     // vectors of a lane in a segment
-constexpr int kLpUnroll = 2;    // segments in flight a warp
+constexpr int kLpRing = 4;      // segment slots of a warp
 constexpr int kLpMaxRanks = 8;  // CTAs of a row
 constexpr int kLpHeld = 512;    // candidates of a CTA (>= 32 a warp)
 constexpr int64_t kLpMaxVocabulary = 1 << 20;
@@ -132,8 +132,9 @@ __device__ __forceinline__ LpPart join_lanes(LpPart p, int count, float c) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs(LpArgs a) {
+__global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
   extern __shared__ float seg_top[];  // largest logit of each segment of the slice, only with a.top
+  __shared__ uint4 ring[kLpWarps * kLpRing * kLpGroup * 32];
   __shared__ uint64_t buffer[kLpHeld];
   __shared__ int held;
   __shared__ LpPart parts[kLpWarps];
@@ -164,12 +165,12 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs(LpArgs a) {
     }
   }
 
-  // One vector of a lane; where a segment does not lie wholly inside the row, element by
-  // element with -inf outside.
+  // One vector of a lane: whole where it lies inside the row, else element by element with
+  // -inf outside.  `inside`: the whole segment lies inside.
   auto whole = [&](int seg) { return seg * kSeg >= shift && (seg + 1) * kSeg <= length; };
   auto load = [&](int seg, int g, bool inside) {
     const int at = seg * kSeg + (g * 32 + lane) * kVec - shift;
-    if (inside) return __ldg(reinterpret_cast<const uint4*>(base + at));
+    if (inside || (at >= 0 && at + kVec <= a.vocabulary)) return __ldg(reinterpret_cast<const uint4*>(base + at));
     constexpr raw kNone = sizeof(raw) == 4 ? (raw)0xff800000u : std::is_same<T, F16>::value ? (raw)0xfc00u : (raw)0xff80u;
     __align__(16) raw e[kVec];
 #pragma unroll
@@ -184,18 +185,13 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs(LpArgs a) {
   float by = c;
   float m = 0.0f;
   unsigned long long s2 = 0, a2 = 0;
-  auto add = [&](int seg, const uint4 (&v)[kLpUnroll][kLpGroup], int count) {
-    float top[kLpUnroll], rise = ninf;
+  auto add = [&](int seg, const uint4 (&v)[kLpGroup]) {
+    float rise = T::largest(v[0]);
 #pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u) {
-      if (u >= count) break;
-      float l = T::largest(v[u][0]);
-#pragma unroll
-      for (int g = 1; g < kLpGroup; ++g) l = max_nan(l, T::largest(v[u][g]));
-      top[u] = warp_largest(l);
-      rise = max_nan(rise, top[u]);
-      if (a.top && lane == 0) seg_top[seg + u * kLpWarps - seg0] = top[u];
-    }
+    for (int g = 1; g < kLpGroup; ++g) rise = max_nan(rise, T::largest(v[g]));
+    rise = warp_largest(rise);
+    if (a.top && lane == 0) seg_top[seg - seg0] = rise;
+    if (rise == ninf) return;  // nothing but masked logits
     if (!(rise <= most)) {  // the same in all lanes
       if (rise < __int_as_float(0x7f800000)) {
         const float last = by;
@@ -213,66 +209,68 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs(LpArgs a) {
       }
     }
 #pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u) {
-      if (u >= count) break;
-      if (top[u] == ninf) continue;  // nothing but masked logits
+    for (int g = 0; g < kLpGroup; ++g) {
+      float f[kVec];
+      T::unpack(v[g], f);
 #pragma unroll
-      for (int g = 0; g < kLpGroup; ++g) {
-        float f[kVec];
-        T::unpack(v[u][g], f);
-#pragma unroll
-        for (int i = 0; i < kVec; i += 2) {
-          const float2 d = f2_unpack(f2_fma(f2_pack(f[i], f[i + 1]), f2_pack(by, by), f2_pack(-m, -m)));
-          const float t0 = fmaxf(d.x, -256.0f), t1 = fmaxf(d.y, -256.0f);  // masked logits: 2^t = 0 and t finite
-          const unsigned long long e = f2_pack(ex2_approx(t0), ex2_approx(t1));
-          s2 = f2_add(s2, e);
-          a2 = f2_fma(e, f2_pack(t0, t1), a2);
-        }
+      for (int i = 0; i < kVec; i += 2) {
+        const float2 d = f2_unpack(f2_fma(f2_pack(f[i], f[i + 1]), f2_pack(by, by), f2_pack(-m, -m)));
+        const float t0 = fmaxf(d.x, -256.0f), t1 = fmaxf(d.y, -256.0f);  // masked logits: 2^t = 0 and t finite
+        const unsigned long long e = f2_pack(ex2_approx(t0), ex2_approx(t1));
+        s2 = f2_add(s2, e);
+        a2 = f2_fma(e, f2_pack(t0, t1), a2);
       }
     }
   };
-  int seg = seg0 + warp;
-  uint4 v[kLpUnroll][kLpGroup];
-  // batches wholly inside the row (all but the row's ends), then the rest segment by segment
-  if (seg < seg1 && !whole(seg)) {
+  auto fetch = [&](int seg, uint4 (&to)[kLpGroup]) {
 #pragma unroll
-    for (int g = 0; g < kLpGroup; ++g) v[0][g] = load(seg, g, false);
-    add(seg, v, 1);
+    for (int g = 0; g < kLpGroup; ++g) to[g] = load(seg, g, false);
+  };
+  // This warp's segments seg, seg + kLpWarps, .. below end: those that the row does not fill (its
+  // first and last at most) are loaded with guards.
+  int seg = seg0 + warp, end = seg1, edge = -1;
+  if (seg < end && !whole(seg)) {
+    edge = seg;
     seg += kLpWarps;
   }
-  constexpr int kBatch = kLpWarps * kLpUnroll;
-  auto fits = [&](int first) {
-    const int last = first + kLpWarps * (kLpUnroll - 1);
-    return last < seg1 && whole(last);
-  };
-  auto fetch = [&](int first, uint4 (&to)[kLpUnroll][kLpGroup]) {
-#pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u)
-#pragma unroll
-      for (int g = 0; g < kLpGroup; ++g) to[u][g] = load(first + u * kLpWarps, g, true);
-  };
-  if (fits(seg)) {  // the next batch's loads are in flight while one is added up
-    uint4 next[kLpUnroll][kLpGroup];
-    fetch(seg, v);
-    while (true) {
-      const bool more = fits(seg + kBatch);
-      if (more) fetch(seg + kBatch, next);
-      add(seg, v, kLpUnroll);
-      seg += kBatch;
-      if (!more) break;
-      const bool again = fits(seg + kBatch);
-      if (again) fetch(seg + kBatch, v);
-      add(seg, next, kLpUnroll);
-      seg += kBatch;
-      if (!again) break;
+  const int final_seg = seg + (end - 1 - seg) / kLpWarps * kLpWarps;
+  if (seg < end && !whole(final_seg)) {
+    if (edge >= 0) {  // both ends
+      uint4 v[kLpGroup];
+      fetch(edge, v);
+      add(edge, v);
     }
+    edge = final_seg;
+    end = final_seg;
   }
-#pragma unroll 1
-  for (; seg < seg1; seg += kLpWarps) {
-    const bool inside = whole(seg);
+  // The others go through a ring of segment slots in shared memory: a lane copies its own
+  // vectors asynchronously and reads them back itself, so nothing but its copies' completion
+  // is waited for, and loads in flight cost no registers.
+  uint4* slot = ring + (warp * kLpRing * kLpGroup) * 32 + lane;
+  const uint4* from = reinterpret_cast<const uint4*>(base + (int64_t)seg * kSeg - shift) + lane;
+  const int whole_segs = seg < end ? (end - seg + kLpWarps - 1) / kLpWarps : 0;
+  auto copy = [&](int i) {
+    if (i < whole_segs) {
 #pragma unroll
-    for (int g = 0; g < kLpGroup; ++g) v[0][g] = load(seg, g, inside);
-    add(seg, v, 1);
+      for (int g = 0; g < kLpGroup; ++g)
+        cp_async16(slot + ((i % kLpRing) * kLpGroup + g) * 32, from + ((int64_t)i * kLpWarps * kLpGroup + g) * 32);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kLpRing - 1; ++i) copy(i);
+  if (edge >= 0) {
+    uint4 v[kLpGroup];
+    fetch(edge, v);
+    add(edge, v);
+  }
+  for (int i = 0; i < whole_segs; ++i) {
+    copy(i + kLpRing - 1);
+    cp_async_wait<kLpRing - 1>();
+    uint4 v[kLpGroup];
+#pragma unroll
+    for (int g = 0; g < kLpGroup; ++g) v[g] = slot[((i % kLpRing) * kLpGroup + g) * 32];
+    add(seg + i * kLpWarps, v);
   }
   const float2 s_halves = f2_unpack(s2), a_halves = f2_unpack(a2);
   LpPart p = {m, s_halves.x + s_halves.y, a_halves.x + a_halves.y, bad ? kAll : order_key(most)};
@@ -381,7 +379,9 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs(LpArgs a) {
 #pragma unroll
     for (int r = 0; r < kLpMaxRanks; ++r)  // all remote reads in flight together
       lists_of[r] = a.top && r < ranks ? cluster.map_shared_rank(cta_list, r)[lane] : 0ull;
-    const LpPart all = join_lanes(*cluster.map_shared_rank(&cta_part, lane & (ranks - 1)), ranks, c);
+    LpPart all = join_lanes(*cluster.map_shared_rank(&cta_part, lane & (ranks - 1)), ranks, c);
+    all.m = __shfl_sync(kAll, all.m, 0);  // one lane's sums, so that a token has one value wherever it is listed
+    all.s = __shfl_sync(kAll, all.s, 0);
 #pragma unroll
     for (int half = kLpMaxRanks / 2; half; half >>= 1)
       if (half < ranks) {
@@ -415,7 +415,7 @@ ttn_status launch_logprobs(const char* name, LpArgs a, cudaStream_t stream) {
   const int segments = (int)((a.vocabulary + T::kVec - 1 + kSeg - 1) / kSeg);  // at the largest shift
   // Few rows: split each over a cluster, as long as a CTA keeps two rounds of its warps.
   int ranks = 1;
-  while (ranks < kLpMaxRanks && a.rows * ranks * 2 <= 2 * sm_count() && segments > ranks * kLpWarps * kLpUnroll) ranks *= 2;
+  while (ranks < kLpMaxRanks && a.rows * ranks * 2 <= 2 * sm_count() && segments > ranks * kLpWarps * 2) ranks *= 2;
   a.slice = (segments + ranks - 1) / ranks;
   const size_t smem = a.top ? (size_t)a.slice * 4 : 0;
   cudaLaunchConfig_t config = {};
