@@ -63,13 +63,6 @@ __device__ __forceinline__ uint64_t entry(uint32_t key, uint32_t place) {
   return key ? (uint64_t)key << 32 | (uint32_t)~place : 0ull;
 }
 
-// The largest value of the warp, NaN if there is one.
-__device__ __forceinline__ float warp_largest(float v) {
-  float r;
-  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 // Sorts one key or entry a lane, largest first (bitonic).  Not inlined, as merge32: code that
 // runs at most once a row should not be long.
 template <typename K>

@@ -14,6 +14,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   return r;
 }
 
+// The largest value of the warp, NaN if there is one.
+__device__ __forceinline__ float warp_largest(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 struct F32 {
   using raw = uint32_t;
   // the largest of a vector's elements, NaN if one is
