@@ -30,7 +30,8 @@ constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kMaxTopK = 16;  // leaves 16 lanes for candidates behind the last choice
 constexpr uint32_t kAll = 0xffffffffu;
 // Two fp32 ranks further apart than kBand * max(1, |rank|) are in the order of their exact
-// 8 * 2^-24 of its value (s <= 1), the bias addition rounds by |rank| 2^-24 more, twice that
+// values: the exp2 and reciprocal approximations (2 ulp each), x - max, the products and the
+// sum's own error leave s within 8 * 2^-24 of its value (s <= 1), the bias addition rounds by |rank| 2^-24 more, twice that
 // for a difference, and a group's sum of two doubles it again: 36 * 2^-24 = 2.2e-6.
 constexpr float kBand = 2.5e-6f;
 
