@@ -82,27 +82,27 @@ def expert_mlp(x, ids, weights, gate_up, down):
     out = torch.zeros(x.shape, dtype=torch.float64)
     err = torch.zeros(x.shape, dtype=torch.float64)
     f32 = 2.0 ** -24
-    for t in range(x.size(0)):
-        for j in range(ids.size(1)):
-            e = int(ids[t, j])
-            if not 0 <= e < num:
+    for j in range(ids.size(1)):  # in the order of the choices
+        for e in range(num):
+            t = torch.where(ids[:, j] == e)[0]
+            if not len(t):
                 continue
             gu, d, v = gate_up[e].double(), down[e].double(), x[t].double()
-            both, size = gu @ v, gu.abs() @ v.abs()
-            g, u = both[:inner], both[inner:]
+            both, size = v @ gu.T, v.abs() @ gu.abs().T
+            g, u = both[:, :inner], both[:, inner:]
             s = g / (1 + torch.exp(-g))
             h = s * u
-            w = float(weights[t, j])
-            y = d @ h
+            w = weights[t, j].double()[:, None]
+            y = h @ d.T
             # a sum of n products: each product and each partial sum rounds once; |silu'| <= 1.1;
             # exp (2 ulp of a value <= 1 + e^-g), the division and the product by u add 8 roundings
-            dh = f32 * ((hidden + 2) * (1.1 * size[:inner] * u.abs() + s.abs() * size[inner:]) + 8 * h.abs())
+            dh = f32 * ((hidden + 2) * (1.1 * size[:, :inner] * u.abs() + s.abs() * size[:, inner:]) + 8 * h.abs())
             dh += half * h.abs() + tiny
-            dy = d.abs() @ (dh + f32 * (inner + 2) * h.abs())
-            pad = torch.nn.functional.pad(y.abs(), (0, -hidden % 32)).view(-1, 32)
-            peak = pad.max(1, keepdim=True).values.expand_as(pad).reshape(-1)[:hidden]
+            dy = (dh + f32 * (inner + 2) * h.abs()) @ d.abs().T
+            pad = torch.nn.functional.pad(y.abs(), (0, -hidden % 32)).view(len(t), -1, 32)
+            peak = pad.max(2, keepdim=True).values.expand_as(pad).reshape(len(t), -1)[:, :hidden]
             out[t] += w * y
-            err[t] += abs(w) * (dy + 2.0 ** -15 * (peak + dy)) + f32 * (ids.size(1) + 2) * abs(w) * y.abs()
+            err[t] += w.abs() * (dy + 2.0 ** -15 * (peak + dy)) + f32 * (ids.size(1) + 2) * w.abs() * y.abs()
     return out, err
 
 

@@ -175,7 +175,9 @@ MLP = [  # tokens, hidden, inner, experts, top_k, dropped, skew
     (1, 8, 16, 1, 1, 0.0, 0.0), (1, 64, 48, 4, 2, 0.0, 0.0), (1, 136, 80, 8, 8, 0.0, 0.0), (3, 256, 128, 5, 3, 0.3, 0.0),
     (2, 1032, 688, 4, 2, 0.0, 0.0), (17, 72, 16, 7, 1, 0.0, 0.0), (40, 264, 112, 6, 4, 0.25, 0.0),
     (129, 64, 64, 3, 2, 0.0, 0.5), (300, 128, 144, 2, 2, 0.1, 0.0), (65, 520, 272, 40, 6, 0.0, 0.05),
-    (600, 40, 32, 4, 3, 0.0, 1.0), (33, 512, 256, 2, 1, 0.0, 3.0), (260, 328, 208, 1, 1, 0.0, 0.0)]
+    (600, 40, 32, 4, 3, 0.0, 1.0), (33, 512, 256, 2, 1, 0.0, 3.0), (260, 328, 208, 1, 1, 0.0, 0.0),
+    # many rows an expert: two sub-tiles in the first product, in the second, in both with ragged runs
+    (2400, 72, 2048, 2, 2, 0.0, 0.3), (4760, 2048, 48, 3, 2, 0.1, 0.4), (5000, 1000, 992, 5, 2, 0.05, 0.2)]
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])

@@ -228,15 +228,19 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan(const int32_t* __res
 
 constexpr int kTileN = 256;      // rows of an expert in a tile, at most
 constexpr int kStepK = 64;       // reduction elements of a ring stage: 128 bytes, the swizzle's width
-constexpr int kStages = 6;
+constexpr int kMaxStages = 6;
+constexpr int ring_stages(int subs) { return subs == 2 ? 4 : kMaxStages; }
 constexpr uint32_t kABytes = 128 * kStepK * 2, kBBytes = kTileN / 2 * kStepK * 2;
-constexpr uint32_t kStageBytes = kABytes + kBBytes;
-constexpr int kEpiWarps = 8;
+constexpr uint32_t kRingBytes = 192 * 1024;
+static_assert(kRingBytes == ring_stages(1) * (kABytes + kBBytes) && kRingBytes == ring_stages(2) * (2 * kABytes + kBBytes),
+              "both rings fill the same space");
+constexpr int epi_warps(bool gate_up) { return gate_up ? 12 : 8; }
 constexpr int kGatherWarps = 4;  // of the first product
 constexpr int kGatherRows = kTileN / 2 / kGatherWarps;
-constexpr int product_threads(bool gather) { return 64 + 32 * kEpiWarps + (gather ? 32 * kGatherWarps : 0); }
-constexpr int kStagingPitch = 36;                          // words: conflict-free both ways
-constexpr uint32_t kStagingBytes = 16 * kStagingPitch * 4;  // one epilogue warp: 16 rows x 32 values (or 32 x 16 halves)
+constexpr int product_threads(bool gate_up) { return 64 + 32 * epi_warps(gate_up) + (gate_up ? 32 * kGatherWarps : 0); }
+constexpr int kStagingPitch = 36;  // words: conflict-free both ways
+// one epilogue warp: 32 rows x 16 activations, or 16 rows x 32 values
+constexpr uint32_t staging_bytes(bool gate_up) { return gate_up ? 32 * 16 * 2 : 16 * kStagingPitch * 4; }
 constexpr int kShareBlock = 32;              // features that share a scale
 
 struct ProductArgs {
@@ -251,8 +255,8 @@ struct ProductArgs {
 struct ProductMaps {
   CUtensorMap a, b;
 };
-__host__ __device__ constexpr uint32_t product_smem(int experts) {
-  return 1024 + kStages * kStageBytes + kEpiWarps * kStagingBytes + 2 * 4 * (uint32_t)(experts + 1);
+__host__ __device__ constexpr uint32_t product_smem(bool gate_up, int experts) {
+  return 1024 + kRingBytes + epi_warps(gate_up) * staging_bytes(gate_up) + 2 * 4 * (uint32_t)(experts + 1);
 }
 
 // Tile t of the list: experts in order, of an expert its runs of rows, of a run its weight rows.
@@ -272,19 +276,29 @@ struct TileList {
   }
 };
 
-// kGateUp: the first product; kGather: its token rows come from x through `order` (else from a sorted copy).
-template <typename T, bool kGateUp, bool kGather>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGather), 1)
+// kGateUp: the first product, whose token rows are gathered from x through `order`.
+// kSubs: weight-row tiles of 256 that share each stage's token rows.  1: two accumulators, so
+// that a tile's epilogue overlaps the next tile's products.  2, for the first product of many
+// rows an expert: a quarter fewer operand bytes a product and half the gathering (TMA takes
+// about 7 cycles a gathered row, 3 a row of a tile); each sub-tile has one accumulator, and the
+// next tile's products begin with sub-tile 0 alone while the epilogue still reads sub-tile 1.
+// 8192 tokens x 8 of 64 experts, hidden 2048, inner 1024: 561 us with one sub-tile, 459 + 55 with
+// one and a sorted copy of x, 438 with two (374 without the epilogue: at 1.6 GHz under the power
+// cap the tensor cores are then the bound).
+template <typename T, bool kGateUp, int kSubs>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGateUp), 1)
     expert_products(ProductArgs a, const __grid_constant__ ProductMaps maps) {
+  constexpr int kStages = ring_stages(kSubs), kEpiWarps = epi_warps(kGateUp), kEpiGroups = kEpiWarps / 4;
+  constexpr uint32_t kStageBytes = kSubs * kABytes + kBBytes;
   extern __shared__ __align__(1024) unsigned char smem[];
-  __shared__ __align__(8) uint64_t bars[2 * kStages + 4];  // full[s], empty[s], acc_full[2], acc_empty[2]
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 4];  // full[s], empty[s], acc_full[2], acc_empty[2]
   __shared__ uint32_t tmem_slot;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
   const uint32_t smem0 = ((uint32_t)__cvta_generic_to_shared(smem) + 1023u) & ~1023u;
   unsigned char* generic0 = smem + (smem0 - (uint32_t)__cvta_generic_to_shared(smem));
-  unsigned char* staging = generic0 + kStages * kStageBytes;
-  int32_t* offsets = reinterpret_cast<int32_t*>(staging + kEpiWarps * kStagingBytes);
+  unsigned char* staging = generic0 + kRingBytes;
+  int32_t* offsets = reinterpret_cast<int32_t*>(staging + kEpiWarps * staging_bytes(kGateUp));
   int32_t* tiles = offsets + a.experts + 1;
   const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(&bars[0]);
   auto full_bar = [&](int s) { return bar0 + 8 * s; };
@@ -345,15 +359,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
           fault = 2;
           break;
         }
-        const uint32_t sa = smem0 + s * kStageBytes, sb = sa + kABytes;
+        const uint32_t sa = smem0 + s * kStageBytes, sb = sa + kSubs * kABytes;
         const uint32_t bar = cluster_addr(full_bar(s), 0);
         if (elect_one()) {
-          if (rank == 0) mbar_expect_tx(full_bar(s), 2 * (kABytes + (uint32_t)half * kStepK * 2));
-          if (kGateUp)
-            tma_pair_load5(sa, &maps.a, step * kStepK, 0, 0, m * 8 + rank * 4, list.e, bar);
-          else
-            tma_pair_load3(sa, &maps.a, step * kStepK, m * 256 + rank * 128, list.e, bar);
-          if (!kGather) {
+          if (rank == 0) mbar_expect_tx(full_bar(s), 2 * (kSubs * kABytes + (uint32_t)half * kStepK * 2));
+#pragma unroll
+          for (int u = 0; u < kSubs; ++u) {
+            const int tile = m * kSubs + u;  // of 256 weight rows: 128 gated features, or 256 outputs
+            if (kGateUp)
+              tma_pair_load5(sa + u * kABytes, &maps.a, step * kStepK, 0, 0, tile * 8 + rank * 4, list.e, bar);
+            else
+              tma_pair_load3(sa + u * kABytes, &maps.a, step * kStepK, tile * 256 + rank * 128, list.e, bar);
+          }
+          if (!kGateUp) {
 #pragma unroll
             for (int i = 0; i < kTileN / 32; ++i)
               if (i * 16 < half)
@@ -364,7 +382,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
         if (++s == kStages) s = 0, phase ^= 1;
       }
     }
-  } else if (kGather && warp >= 2 + kEpiWarps) {
+  } else if (kGateUp && warp >= 2 + kEpiWarps) {
     // Gathering warps, one thread each: every fourth copy of four rows.  A stage has 16 rows at
     // least, so each warp has a part in every stage: none falls two phases of a barrier
     // behind, where parities repeat.
@@ -386,7 +404,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
           fault = 2;
           break;
         }
-        const uint32_t sb = smem0 + s * kStageBytes + kABytes + line * kStepK * 2;
+        const uint32_t sb = smem0 + s * kStageBytes + kSubs * kABytes + line * kStepK * 2;
         const uint32_t bar = cluster_addr(full_bar(s), 0);
         if (elect_one()) {
 #pragma unroll
@@ -408,124 +426,168 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
         list.at(t, m, row0, rows);
         // operand format: 0 = fp16, 1 = bf16, the same for both
         const uint32_t idesc = umma_idesc(256, (rows + 31) & ~31, false, false) | (a.bf16 ? 1u << 7 | 1u << 10 : 0u);
-        const int acc = j & 1;
-        if (!__all_sync(kAll, mbar_wait_cluster<true>(acc_empty(acc), ((j >> 1) & 1) ^ 1))) {
+        // kSubs 1: accumulator j & 1, filled every second tile; 2: accumulator u of sub-tile u, every tile
+        const int acc = kSubs == 1 ? j & 1 : 0;
+        const uint32_t turn = (uint32_t)(kSubs == 1 ? j >> 1 : j) & 1;
+        if (!__all_sync(kAll, mbar_wait_cluster<true>(acc_empty(acc), turn ^ 1))) {
           fault = 4;
           break;
         }
-        const uint32_t d = tmem + acc * kTileN;
+        auto multiply = [&](int u, int stage, bool add) {  // of one stage into one accumulator
+          const uint32_t base = smem0 + stage * kStageBytes;
+          const uint64_t da = smem_desc(base + u * kABytes, 16, 1024, kSwizzle128B);
+          const uint64_t db = smem_desc(base + kSubs * kABytes, 16, 1024, kSwizzle128B);
+          const uint32_t d = tmem + (kSubs == 1 ? acc : u) * kTileN;
+#pragma unroll
+          for (int k = 0; k < kStepK / 16; ++k)  // 16 elements: 32 bytes along the swizzled rows
+            umma_pair_ss(d, da + 2 * k, db + 2 * k, idesc, add || k > 0);
+        };
+        int held = 0;        // kSubs 2: stages up to this one that sub-tile 1 has not taken yet
+        bool open = false;   // and whether its accumulator is free
         for (int step = 0; step < a.steps; ++step) {
           if (!__all_sync(kAll, mbar_wait_cluster<true>(full_bar(s), phase))) {
             fault = 1;
             break;
           }
           tc_fence_after();
-          const uint64_t da = smem_desc(smem0 + s * kStageBytes, 16, 1024, kSwizzle128B);
-          const uint64_t db = smem_desc(smem0 + s * kStageBytes + kABytes, 16, 1024, kSwizzle128B);
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < kStepK / 16; ++k)  // 16 elements: 32 bytes along the swizzled rows
-              umma_pair_ss(d, da + 2 * k, db + 2 * k, idesc, step > 0 || k > 0);
-            umma_pair_commit(empty_bar(s));
-            if (step == a.steps - 1) umma_pair_commit(acc_full(acc));
+          const bool last = step == a.steps - 1;
+          if (kSubs == 1) {
+            if (elect_one()) {
+              multiply(0, s, step > 0);
+              umma_pair_commit(empty_bar(s));
+              if (last) umma_pair_commit(acc_full(acc));
+            }
+          } else {
+            if (elect_one()) {
+              multiply(0, s, step > 0);
+              if (last) umma_pair_commit(acc_full(0));
+            }
+            __syncwarp();
+            ++held;
+            if (!open) {
+              const bool must = last || held == kStages;  // nothing more can be loaded before
+              open = __all_sync(kAll, must ? mbar_wait_cluster<true>(acc_empty(1), turn ^ 1)
+                                           : mbar_test_cluster(acc_empty(1), turn ^ 1));
+              if (must && !open) {
+                fault = 4;
+                break;
+              }
+              tc_fence_after();
+            }
+            if (open) {
+              int stage = s - (held - 1);
+              if (stage < 0) stage += kStages;
+              for (; held; --held) {
+                if (elect_one()) {
+                  multiply(1, stage, step - (held - 1) > 0);
+                  umma_pair_commit(empty_bar(stage));
+                }
+                __syncwarp();
+                if (++stage == kStages) stage = 0;
+              }
+              if (last && elect_one()) umma_pair_commit(acc_full(1));
+            }
           }
           __syncwarp();
           if (++s == kStages) s = 0, phase ^= 1;
         }
       }
     }
-  } else if (warp < 2 + kEpiWarps) {  // epilogue: TMEM lanes 32 (warp % 4).., every second 32-column chunk
+  } else if (warp < 2 + kEpiWarps) {  // epilogue: TMEM lanes 32 (warp % 4).., every kEpiGroups-th chunk of columns
     const int quarter = warp & 3, group = (warp - 2) >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    unsigned char* own = staging + (warp - 2) * kStagingBytes;
+    unsigned char* own = staging + (warp - 2) * staging_bytes(kGateUp);
     int j = 0;
-    for (int t = first; t < count; t += stride, ++j) {
+    for (int t = first; t < count && !fault; t += stride, ++j) {
       int m, row0, rows;
       list.at(t, m, row0, rows);
-      const int acc = j & 1;
-      if (!__all_sync(kAll, mbar_wait_cluster<false>(acc_full(acc), (j >> 1) & 1))) {
-        fault = 4;
-        break;
-      }
-      tc_fence_after();
-      if (kGateUp) {
-        const int f0 = m * 128 + (int)rank * 64 + quarter * 16;
-        const bool low = lane < 16;
-        uint16_t* out = reinterpret_cast<uint16_t*>(own) + (low ? 0 : 16) + (lane & 15);
-        for (int c = group * 32; c < rows && f0 < a.rows; c += 64) {  // a.rows is a multiple of 16
-          uint32_t r[32];
-          tmem_ld32(lanes + acc * kTileN + c, r);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {  // lanes below 16 take column 2i, the others 2i + 1
-            const float even = __uint_as_float(r[2 * i]), odd = __uint_as_float(r[2 * i + 1]);
-            const float other = __shfl_xor_sync(kAll, low ? odd : even, 16);
-            const float g = low ? even : other, u = low ? other : odd;
-            out[i * 32] = T::round(__fdividef(g, 1.0f + __expf(-g)) * u);
-          }
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {  // two lanes a row: whole 32-byte sectors
-            const int n = i * 16 + (lane >> 1), q = lane & 1;
-            if (c + n < rows)
-              reinterpret_cast<uint4*>(a.h + (int64_t)(row0 + c + n) * a.rows + f0)[q] =
-                  reinterpret_cast<const uint4*>(own)[n * 2 + q];
-          }
-          __syncwarp();
+#pragma unroll 1
+      for (int u = 0; u < kSubs; ++u) {
+        const int acc = kSubs == 1 ? j & 1 : u, tile = m * kSubs + u;
+        if (!__all_sync(kAll, mbar_wait_cluster<false>(acc_full(acc), (uint32_t)(kSubs == 1 ? j >> 1 : j) & 1))) {
+          fault = 4;
+          break;
         }
-      } else {
-        // 16 columns at a time through shared memory: two lanes a row then hold 16 neighbouring
-        // features each, so the row's largest is found in registers (a warp-wide reduction a
-        // column made this epilogue 200 cycles a column and the product 434 us, now 215 us).
-        const int f0 = m * 256 + (int)rank * 128 + quarter * 32;
-        const int n = lane >> 1, f = f0 + (lane & 1) * 16;
-        uint32_t* in = reinterpret_cast<uint32_t*>(own) + lane;
-        const uint4* back = reinterpret_cast<const uint4*>(own) + (n * kStagingPitch + (lane & 1) * 16) / 4;
-        for (int c = group * 16; c < rows && f0 < a.rows; c += 32) {
-          const int pair = c + n < rows ? a.order[row0 + c + n] : -1;
-          uint32_t r[16];
-          tmem_ld16(lanes + acc * kTileN + c, r);
+        tc_fence_after();
+        if (kGateUp) {
+          const int f0 = tile * 128 + (int)rank * 64 + quarter * 16;
+          const bool low = lane < 16;
+          uint16_t* out = reinterpret_cast<uint16_t*>(own) + (low ? 0 : 16) + (lane & 15);
+          for (int c = group * 32; c < rows && f0 < a.rows; c += kEpiGroups * 32) {  // a.rows is a multiple of 16
+            uint32_t r[32];
+            tmem_ld32(lanes + acc * kTileN + c, r);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) in[i * kStagingPitch] = r[i];
-          __syncwarp();
-          uint32_t v[16], top = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 q = back[i];
-            v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
-          }
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) top = max(top, v[i] & 0x7fffffffu);
-          top = max(top, __shfl_xor_sync(kAll, top, 1));
-          const float peak = __uint_as_float(top);
-          const bool whole = peak >= 1e-30f && top < 0x7f800000u;
-          const float inverse = __fdividef(32767.0f, peak);
-          uint32_t w[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float lo = __uint_as_float(v[2 * i]), hi = __uint_as_float(v[2 * i + 1]);
-            w[i] = __byte_perm(__float2int_rn(lo * inverse), __float2int_rn(hi * inverse), 0x5410);
-          }
-          if (!whole) {  // zeros, vanishing values, infinities, NaN: as bf16
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = BF16::round2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-          }
-          if (pair >= 0) {
-            if ((lane & 1) == 0) a.scale[(int64_t)pair * a.blocks + f0 / kShareBlock] = whole ? peak * (1.0f / 32767.0f) : -1.0f;
-            int16_t* to = a.share + (int64_t)pair * a.rows + f;
-            if (a.wide) {  // rows of whole 32-byte sectors
-              if (f < a.rows) store32(to, w);
-            } else {
-              if (f < a.rows) reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-              if (f + 8 < a.rows) reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            for (int i = 0; i < 16; ++i) {  // lanes below 16 take column 2i, the others 2i + 1
+              const float even = __uint_as_float(r[2 * i]), odd = __uint_as_float(r[2 * i + 1]);
+              const float other = __shfl_xor_sync(kAll, low ? odd : even, 16);
+              const float g = low ? even : other, u = low ? other : odd;
+              out[i * 32] = T::round(__fdividef(g, 1.0f + __expf(-g)) * u);
             }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {  // two lanes a row: whole 32-byte sectors
+              const int n = i * 16 + (lane >> 1), q = lane & 1;
+              if (c + n < rows)
+                reinterpret_cast<uint4*>(a.h + (int64_t)(row0 + c + n) * a.rows + f0)[q] =
+                    reinterpret_cast<const uint4*>(own)[n * 2 + q];
+            }
+            __syncwarp();
           }
-          __syncwarp();
+        } else {
+          // 16 columns at a time through shared memory: two lanes a row then hold 16 neighbouring
+          // features each, so the row's largest is found in registers (a warp-wide reduction a
+          // column made this epilogue 200 cycles a column and the product 434 us, now 215 us).
+          const int f0 = tile * 256 + (int)rank * 128 + quarter * 32;
+          const int n = lane >> 1, f = f0 + (lane & 1) * 16;
+          uint32_t* in = reinterpret_cast<uint32_t*>(own) + lane;
+          const uint4* back = reinterpret_cast<const uint4*>(own) + (n * kStagingPitch + (lane & 1) * 16) / 4;
+          for (int c = group * 16; c < rows && f0 < a.rows; c += kEpiGroups * 16) {
+            const int pair = c + n < rows ? a.order[row0 + c + n] : -1;
+            uint32_t r[16];
+            tmem_ld16(lanes + acc * kTileN + c, r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) in[i * kStagingPitch] = r[i];
+            __syncwarp();
+            uint32_t v[16], top = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint4 q = back[i];
+              v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = max(top, v[i] & 0x7fffffffu);
+            top = max(top, __shfl_xor_sync(kAll, top, 1));
+            const float peak = __uint_as_float(top);
+            const bool whole = peak >= 1e-30f && top < 0x7f800000u;
+            const float inverse = __fdividef(32767.0f, peak);
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float lo = __uint_as_float(v[2 * i]), hi = __uint_as_float(v[2 * i + 1]);
+              w[i] = __byte_perm(__float2int_rn(lo * inverse), __float2int_rn(hi * inverse), 0x5410);
+            }
+            if (!whole) {  // zeros, vanishing values, infinities, NaN: as bf16
+#pragma unroll
+              for (int i = 0; i < 8; ++i) w[i] = BF16::round2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+            }
+            if (pair >= 0) {
+              if ((lane & 1) == 0) a.scale[(int64_t)pair * a.blocks + f0 / kShareBlock] = whole ? peak * (1.0f / 32767.0f) : -1.0f;
+              int16_t* to = a.share + (int64_t)pair * a.rows + f;
+              if (a.wide) {  // rows of whole 32-byte sectors
+                if (f < a.rows) store32(to, w);
+              } else {
+                if (f < a.rows) reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                if (f + 8 < a.rows) reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+              }
+            }
+            __syncwarp();
+          }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty(acc), 0));
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty(acc), 0));
     }
   }
   if (fault) {
@@ -539,22 +601,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
   cluster_barrier();
   tc_fence_after();
   if (warp == 1) tmem_pair_dealloc(tmem, 2 * kTileN);
-}
-
-// The rows of x in the order of the sorted pairs: one warp a row, 16 bytes a lane.
-constexpr int kSortThreads = 256;
-__global__ void __launch_bounds__(kSortThreads) expert_sort_rows(const uint16_t* __restrict__ x, int64_t x_stride,
-                                                                 int hidden, int top_k, const int32_t* __restrict__ count,
-                                                                 const int32_t* __restrict__ order,
-                                                                 uint16_t* __restrict__ sorted) {
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, row = blockIdx.x * (kSortThreads / 32) + (threadIdx.x >> 5);
-  if (row >= *count) return;
-  const uint4* from = reinterpret_cast<const uint4*>(x + (int64_t)(order[row] / top_k) * x_stride);
-  uint4* to = reinterpret_cast<uint4*>(sorted + (int64_t)row * hidden);
-#pragma unroll 4
-  for (int i = lane; i < hidden / 8; i += 32) to[i] = __ldg(from + i);
 }
 
 // out[token] = sum of weight * share over the token's choices, in their order; 8 features a thread.
@@ -612,17 +658,21 @@ __global__ void __launch_bounds__(kCombineThreads) expert_combine(ExpertArgs a, 
 // experts, hidden 1032, inner 688, 2 choices: 16 pairs 14 us (22), 32 pairs 23.3 (23.7).
 constexpr int64_t kRowsPairs = 32;
 
-// From this many pairs an expert on (on the average), x is copied in sorted order first: the
-// copy costs its bytes, gathering 27 cycles a CTA for four rows of a step, which is hidden
-// until the products bound the step.  64 experts, hidden 2048, inner 1024, 8 choices, with
-// and without the copy: 1024 tokens (128 rows) 195 / 198 us, 2048 tokens 276 / 284, 4096
-// tokens 466 / 491; 10 experts, hidden 1032, inner 688, 140 rows: 37.4 / 34.5 us.
-constexpr int64_t kSortRows = 256;
+// Whether the first product takes two sub-tiles: experts with many rows, no more padding of
+// the weight rows, and tiles enough for every pair of SMs.  64 experts, hidden 2048, inner 1024,
+// 8 choices, both products: 1024 tokens (128 rows an expert) 198.5 us with two, 198.8 with one,
+// 2048 tokens 264 / 287, 4096 tokens 437 / 487.  (The second one does not gain: its
+// sub-tiles take half as many steps, and their longer epilogues then stand alone, 345 us
+// against 258 at 8192 tokens x 8 of 64 experts, hidden 2048, inner 1024.)
+constexpr int64_t kSubRows = 128;
+bool two_subs(int64_t pairs, int64_t experts, int64_t inner) {
+  const int64_t tiles = (inner + 127) / 128;
+  return pairs >= kSubRows * experts && tiles % 2 == 0 && pairs / kTileN * (tiles / 2) >= 2 * (sm_count() / 2);
+}
 
 struct Sizes {
   int64_t pairs, blocks;
   bool rows;                                 // the few-pairs kernels
-  bool gather;                               // the first product gathers its rows
   int64_t order, h, share, scale, total;     // byte offsets into the workspace (offsets at 0)
 };
 bool sizes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64_t top_k, Sizes* s) {
@@ -633,7 +683,6 @@ bool sizes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64
   s->pairs = tokens * top_k;
   s->blocks = (hidden + kShareBlock - 1) / kShareBlock;
   s->rows = s->pairs <= kRowsPairs;
-  s->gather = s->pairs < kSortRows * experts;
   if (s->rows) {
     s->order = s->h = s->share = s->scale = 0;
     s->total = pad(s->pairs * inner * 4);
@@ -675,17 +724,11 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     const cuuint32_t box[5] = {kStepK, 16, 2, 4, 1};
     TTN_TRY(encode_map(name, &gate.a, bf16, 5, a.gate_up, dims, str, box));
   }
-  uint16_t* sorted = (uint16_t*)(ws + s.share);  // read before the shares are written
-  if (s.gather) {  // x: one row a box, four rows a gather
+  {  // x: one row a box, four rows a gather
     const cuuint64_t dims[2] = {hidden, (cuuint64_t)a.tokens};
     const cuuint64_t str[1] = {(cuuint64_t)a.x_stride * 2};
     const cuuint32_t box[2] = {kStepK, 1};
     TTN_TRY(encode_map(name, &gate.b, bf16, 2, a.x, dims, str, box));
-  } else {
-    const cuuint64_t dims[2] = {hidden, (cuuint64_t)s.pairs};
-    const cuuint64_t str[1] = {hidden * 2};
-    const cuuint32_t box[2] = {kStepK, 16};
-    TTN_TRY(encode_map(name, &gate.b, bf16, 2, sorted, dims, str, box));
   }
   {
     const cuuint64_t dims[3] = {inner, hidden, experts};
@@ -703,8 +746,9 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
                                 (int)s.pairs, a.experts, (int)((uintptr_t)a.ids % 16 == 0), offsets, order),
                      name));
   const int64_t runs = s.pairs / kTileN + (s.pairs < a.experts ? s.pairs : a.experts);  // at most
-  const uint32_t smem = product_smem(a.experts);
-  auto products = [&](auto kernel, const ProductMaps& maps, int rows, int length, int tile, int threads) {
+  auto products = [&](auto kernel, bool gate_up, int subs, const ProductMaps& maps, int rows, int length) {
+    const int tile = (gate_up ? 128 : 256) * subs;  // features of a tile
+    const uint32_t smem = product_smem(gate_up, a.experts);
     ProductArgs p = {};
     p.offsets = offsets, p.order = order, p.h = h, p.share = share, p.scale = scale;
     p.experts = a.experts, p.top_k = a.top_k, p.rows = rows;
@@ -717,19 +761,13 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     TTN_TRY(ensure_dynamic_smem((const void*)kernel, (int)smem));
     const int64_t pairs_of_sms = sm_count() / 2, most = runs * p.m_tiles;
     const unsigned grid = 2 * (unsigned)(most < pairs_of_sms ? most : pairs_of_sms);
-    return cuda_check(launch_pdl(kernel, dim3(grid), dim3(threads), smem, stream, p, maps), name);
+    return cuda_check(launch_pdl(kernel, dim3(grid), dim3(product_threads(gate_up)), smem, stream, p, maps), name);
   };
-  if (s.gather) {
-    TTN_TRY(products(expert_products<T, true, true>, gate, a.inner, a.hidden, 128, product_threads(true)));
-  } else {
-    constexpr int kRows = kSortThreads / 32;
-    TTN_TRY(cuda_check(launch_pdl(expert_sort_rows, dim3((unsigned)((s.pairs + kRows - 1) / kRows)), dim3(kSortThreads), 0,
-                                  stream, a.x, a.x_stride, a.hidden, a.top_k, (const int32_t*)(offsets + a.experts),
-                                  (const int32_t*)order, sorted),
-                       name));
-    TTN_TRY(products(expert_products<T, true, false>, gate, a.inner, a.hidden, 128, product_threads(false)));
-  }
-  TTN_TRY(products(expert_products<T, false, false>, down, a.hidden, a.inner, 256, product_threads(false)));
+  if (two_subs(s.pairs, a.experts, a.inner))
+    TTN_TRY(products(expert_products<T, true, 2>, true, 2, gate, a.inner, a.hidden));
+  else
+    TTN_TRY(products(expert_products<T, true, 1>, true, 1, gate, a.inner, a.hidden));
+  TTN_TRY(products(expert_products<T, false, 1>, false, 1, down, a.hidden, a.inner));
   const int64_t items = a.tokens * (a.hidden / 8);
   if (items + kCombineThreads > UINT32_MAX) return fail(TTN_UNSUPPORTED, "%s: output too large", name);
   return cuda_check(launch_pdl(expert_combine<T>, dim3((unsigned)((items + kCombineThreads - 1) / kCombineThreads)),

@@ -220,6 +220,17 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t mbar, uint32_t phase)
     }
   }
 }
+// Whether that phase is over already.
+__device__ __forceinline__ bool mbar_test_cluster(uint32_t mbar, uint32_t phase) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(mbar), "r"(phase)
+      : "memory");
+  return done != 0;
+}
 // Tile loads into this CTA's shared memory, completing on a barrier of either CTA of the
 // pair (`cluster_mbar` from cluster_addr).
 __device__ __forceinline__ void tma_pair_load2(uint32_t dst, const CUtensorMap* map, int c0, int c1,
