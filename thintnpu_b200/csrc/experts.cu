@@ -60,6 +60,7 @@ constexpr int kRowsBlock = kRowsThreads / 32 * kRowsFeatures;
 
 template <typename T>
 __global__ void __launch_bounds__(kRowsThreads) expert_rows_gate_up(ExpertArgs a, float* __restrict__ h, int blocks) {
+  pdl_trigger();  // started after all earlier work: only expert_rows_down overlaps it
   const int64_t pair = blockIdx.x / blocks;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int f0 = (int)(blockIdx.x % blocks) * kRowsBlock + warp * kRowsFeatures;
@@ -109,20 +110,33 @@ __global__ void __launch_bounds__(kDownWarps * 32) expert_rows_down(ExpertArgs a
   const int64_t token = blockIdx.x / blocks;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int d0 = (int)(blockIdx.x % blocks) * kDownRows;  // hidden % 8 == 0: all rows exist
+  bool waited = false;
   for (int j = warp; j < a.top_k; j += blockDim.x >> 5) {
     const int64_t pair = token * a.top_k + j;
     const int e = a.ids[pair];
     float acc[kDownRows] = {};
     const bool live = (unsigned)e < (unsigned)a.experts;
+    const uint16_t* w = a.down + ((int64_t)(live ? e : 0) * a.hidden + d0) * a.inner;
+    const float* hp = h + pair * a.inner;
+    uint4 next[kDownRows];
+    auto fetch = [&](int k) {
+#pragma unroll
+      for (int i = 0; i < kDownRows; ++i)
+        next[i] = live && k < a.inner ? __ldg(reinterpret_cast<const uint4*>(w + (int64_t)i * a.inner + k))
+                                      : make_uint4(0, 0, 0, 0);
+    };
+    fetch(lane * 8);
+    if (!waited) {  // the weights are read while expert_rows_gate_up still runs, its h is not
+      pdl_wait();
+      waited = true;
+    }
     if (live) {
-      const uint16_t* w = a.down + ((int64_t)e * a.hidden + d0) * a.inner;
-      const float* hp = h + pair * a.inner;
 #pragma unroll 2
       for (int k = lane * 8; k < a.inner; k += 256) {
         uint4 v[kDownRows];
 #pragma unroll
-        for (int i = 0; i < kDownRows; ++i)
-          v[i] = __ldg(reinterpret_cast<const uint4*>(w + (int64_t)i * a.inner + k));
+        for (int i = 0; i < kDownRows; ++i) v[i] = next[i];
+        fetch(k + 256);
         const float4 h0 = *reinterpret_cast<const float4*>(hp + k), h1 = *reinterpret_cast<const float4*>(hp + k + 4);
         const float hs[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w};
 #pragma unroll
@@ -787,8 +801,9 @@ ttn_status launch_experts(const char* name, const ExpertArgs& a, const Sizes& s,
   expert_rows_gate_up<T><<<(unsigned)(pairs * gate_blocks), kRowsThreads, 0, stream>>>(a, h, gate_blocks);
   TTN_TRY(launch_check(name));
   const int warps = a.top_k < kDownWarps ? a.top_k : kDownWarps;
-  expert_rows_down<T><<<(unsigned)(a.tokens * down_blocks), warps * 32, 0, stream>>>(a, h, down_blocks);
-  return launch_check(name);
+  return cuda_check(launch_pdl(expert_rows_down<T>, dim3((unsigned)(a.tokens * down_blocks)), dim3(warps * 32), 0,
+                               stream, a, (const float*)h, down_blocks),
+                    name);
 }
 
 }  // namespace
