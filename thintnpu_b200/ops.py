@@ -677,8 +677,8 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     if not 1 <= top_k <= experts:
         _fail(f"{what}: top_k must be in [1, experts]")
     if out is None:
-        weights = torch.empty((rows, top_k), dtype=torch.float32, device=device)
-        ids = torch.empty((rows, top_k), dtype=torch.int32, device=device)
+        weights = logits.new_empty((rows, top_k), dtype=torch.float32)
+        ids = logits.new_empty((rows, top_k), dtype=torch.int32)
     else:
         weights, ids = out
         _like_output(weights, (rows, top_k), torch.float32, device, "route_experts: out weights")
@@ -729,13 +729,13 @@ def expert_mlp(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, ga
     _like_output(experts, (tokens, top_k), torch.int32, device, "expert_mlp: experts")
     _like_output(weights, (tokens, top_k), torch.float32, device, "expert_mlp: weights")
     if out is None:
-        out = torch.empty((tokens, hidden), dtype=dtype, device=device)
+        out = x.new_empty((tokens, hidden))
     elif not (out.shape == x.shape and out.dtype == dtype and out.device == device
               and (out.stride(1) == 1 or hidden == 1)):
         _fail(f"{what}: out must match x, with unit-stride rows")
     if workspace is None:
         need = expert_mlp_workspace_size(tokens, hidden, inner, num, top_k)
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        workspace = x.new_empty(need, dtype=torch.uint8)
     elif not (workspace.dtype == torch.uint8 and workspace.device == device and workspace.is_contiguous()):
         _fail(f"{what}: workspace must be contiguous uint8 on x's device")
     _call_on(device, "ttn_expert_mlp", _ROW_DTYPES[dtype], x.data_ptr(), x.stride(0), tokens, hidden,
@@ -771,10 +771,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     top = int(top)
     if not 0 <= top <= logits.size(1):
         _fail(f"{what}: top must be in [0, vocabulary]")
-    logprobs = torch.empty(rows, dtype=torch.float32, device=device)
-    entropy = torch.empty(rows, dtype=torch.float32, device=device)
-    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
-    top_tokens = torch.empty((rows, top), dtype=torch.int32, device=device)
+    logprobs = logits.new_empty(rows, dtype=torch.float32)
+    entropy = logits.new_empty(rows, dtype=torch.float32)
+    top_logprobs = logits.new_empty((rows, top), dtype=torch.float32)
+    top_tokens = logits.new_empty((rows, top), dtype=torch.int32)
     _call_on(device, "ttn_token_logprobs", _ref(d), tokens.data_ptr(), scale, top, logprobs.data_ptr(),
              entropy.data_ptr(), top_logprobs.data_ptr() if top else None, top_tokens.data_ptr() if top else None)
     return logprobs, entropy, top_logprobs, top_tokens
