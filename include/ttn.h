@@ -446,9 +446,11 @@ ttn_status ttn_token_logprobs(const ttn_tensor* logits, const int64_t* tokens, f
  * dtype TTN_F16 or TTN_BF16 for x, gate_up, down and out.  Ids outside 0..num_experts-1
  * (-1: no choice; another rank's experts) add nothing; a token without any other id
  * gets zeros.  Products accumulate in FP32; the gated activations are rounded to dtype
- * between the two products where the tensor cores take them, nothing else is rounded
- * before out.  hidden % 8 == 0, inner % 16 == 0, 16-byte aligned bases, row strides
- * multiples of 8; tokens * top_k < 2^31 / 256, top_k 1..32.  workspace: at least
+ * between the two products where the tensor cores take them (so they have to lie in its
+ * range), and each pair's share of an output to 2^-15 of the largest of its 32 neighbours;
+ * with up to 32 pairs neither.  hidden % 8 == 0, inner % 16 == 0 (both up to 2^20),
+ * num_experts 1..1024, top_k 1..32, tokens * top_k <= (2^31 - 1) / 256; 16-byte aligned
+ * bases, row strides multiples of 8 and at least hidden.  workspace: at least
  * ttn_expert_mlp_workspace_size bytes (0 for malformed sizes), 256-byte aligned, used by
  * one call at a time. */
 size_t ttn_expert_mlp_workspace_size(int64_t tokens, int64_t hidden, int64_t inner, int64_t num_experts,
@@ -462,6 +464,12 @@ ttn_status ttn_expert_mlp(int dtype, const void* x, int64_t x_row_stride, int64_
  * up waiting (1 = an operand copy, 2 = a free ring stage, 4 = an accumulator); its
  * output is then incomplete.  Synchronous. */
 ttn_status ttn_expert_mlp_fault(uint32_t* fault);
+
+/* Test hook for the bounded waits above: the next ttn_expert_mlp call that takes the
+ * tensor cores issues no operand copy in its first product, whose other roles then give
+ * up after their 200 ms limit and set their bits (1 | 4); nothing stays in flight, and
+ * that call's output is meaningless. */
+void ttn_expert_mlp_test_withhold_copies(void);
 
 #ifdef __cplusplus
 }

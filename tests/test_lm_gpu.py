@@ -254,6 +254,58 @@ def test_mlp_is_deterministic_and_order_free(device):
     assert torch.equal(first[perm].view(torch.int16), moved.view(torch.int16))
 
 
+@pytest.mark.parametrize("tokens", [5, 130])
+def test_mlp_given_workspace_and_odd_addresses(device, tokens):
+    """Ids and weights at addresses that are only 4-byte aligned, and a workspace of the
+    caller's, larger than needed and dirty."""
+    import thintnpu_b200 as ttn
+    args = mlp_inputs(tokens, 96, 48, 5, 3, torch.bfloat16, 31, dropped=0.1)
+    x, ids, weights, gate_up, down = (t.to(device) for t in args)
+    odd_ids = torch.empty(tokens * 3 + 1, dtype=torch.int32, device=device)[1:].view(tokens, 3)
+    odd_weights = torch.empty(tokens * 3 + 1, device=device)[1:].view(tokens, 3)
+    odd_ids.copy_(ids)
+    odd_weights.copy_(weights)
+    need = ttn.ops.expert_mlp_workspace_size(tokens, 96, 48, 5, 3)
+    workspace = torch.full((need + 512,), 255, dtype=torch.uint8, device=device)
+    for _ in range(2):
+        check_mlp(ttn.expert_mlp(x, odd_ids, odd_weights, gate_up, down, workspace=workspace), args)
+    assert bool((workspace[need:] == 255).all())
+
+
+def test_mlp_two_streams_at_once(device):
+    import thintnpu_b200 as ttn
+    sets = [[t.to(device) for t in mlp_inputs(700, 256, 128, 6, 2, torch.float16, seed)] for seed in (1, 2)]
+    want = [ttn.expert_mlp(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(ttn.expert_mlp(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert torch.equal(g.view(torch.int16), want[i].view(torch.int16))
+    assert ttn.ops.expert_mlp_fault() == 0
+
+
+def test_mlp_bounded_waits_run_out_and_the_next_call_is_right(device):
+    """A call whose first product gets no operands gives up within its limits and says why;
+    the context and the next call are unharmed."""
+    import thintnpu_b200 as ttn
+    from thintnpu_b200 import _lib
+    args = mlp_inputs(200, 128, 64, 4, 2, torch.bfloat16, 3)
+    dev = [t.to(device) for t in args]
+    assert ttn.ops.expert_mlp_fault() == 0
+    _lib.lib().ttn_expert_mlp_test_withhold_copies()
+    ttn.expert_mlp(*dev)
+    torch.cuda.synchronize()
+    assert ttn.ops.expert_mlp_fault() == 5
+    check_mlp(ttn.expert_mlp(*dev), args)
+    assert ttn.ops.expert_mlp_fault() == 0
+
+
 # ------------------------------------------------------------------ token_logprobs
 
 def check_logprobs(device, logits, tokens, top, scale=1.0, dev_logits=None):
@@ -346,6 +398,41 @@ def test_logprobs_large_vocabulary_and_empty(device):
     assert [tuple(t.shape) for t in out] == [(0,), (0,), (0, 3), (0, 3)]
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_logprobs_few_left_and_equal_rows(device, dtype):
+    """Rows under a narrow mask (fewer tokens left than the alternatives asked for, spread over
+    the vocabulary), constant rows, and rows that rise or fall by the finest steps."""
+    g = torch.Generator().manual_seed(12)
+    v = 20011
+    rows = torch.full((8, v), -math.inf)
+    for r, left in ((0, 3), (1, 40)):
+        at = torch.randperm(v, generator=g)[:left]
+        rows[r, at] = torch.randn(left, generator=g)
+    rows[2] = 0.0
+    rows[3] = torch.finfo(DTYPES[dtype]).min
+    rows[4, ::2] = 1.5
+    rows[5] = torch.arange(v) * 2.0 ** -10
+    rows[6] = torch.arange(v).flip(0) * 2.0 ** -10
+    rows[7, -1] = -2.0
+    tokens = torch.randint(v, (8,), generator=g)
+    for top in (1, 20, 32):
+        check_logprobs(device, rows.to(DTYPES[dtype]), tokens, top)
+
+
+def test_logprobs_many_rows_of_the_largest_vocabulary(device):
+    """One CTA a row holds every segment maximum of a 2^20 vocabulary: more than 48 KB of
+    shared memory (the rows are one row, expanded)."""
+    import thintnpu_b200 as ttn
+    g = torch.Generator().manual_seed(14)
+    row = (torch.randn(1, 1 << 20, generator=g) * 2).float()
+    want = lm.token_logprobs(row, torch.tensor([77]), 20)
+    got = ttn.token_logprobs(row.to(device).expand(400, -1), torch.full((400,), 77).to(device), top=20)
+    assert torch.equal(got[3].cpu(), want[3].expand(400, -1))
+    bound = (8 * (want[2].abs() + math.log(1 << 20)) + (1 << 20) / 256 + 64) * U
+    assert bool(((got[2].cpu().double() - want[2]).abs() <= bound).all())
+    assert torch.equal(got[0], got[0][:1].expand(400))
+
+
 # ------------------------------------------------------------------ together
 
 def _layer(ttn, x, router, bias, gate_up, down, head, tokens):
@@ -376,6 +463,7 @@ def test_layer_and_read_out_eager_captured_and_on_another_stream(device, tokens)
                                 renormalize=True)
     assert torch.equal(eager[4].cpu(), want_ids)
     out = ttn.expert_mlp(x, eager[4], eager[5], gate_up, down)
+    assert ttn.ops.expert_mlp_fault() == 0
     check_mlp(out, tuple(t.cpu() for t in (x, eager[4], eager[5], gate_up, down)))
     check_logprobs(device, (eager[6] @ head).cpu(), given.cpu(), 3)
 

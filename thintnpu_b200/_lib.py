@@ -38,7 +38,7 @@ EXPORTS = (
     "ttn_conv2d_fault_f16", "ttn_conv2d_test_withhold_copies", "ttn_depthwise_nc1hwc0_f16",
     "ttn_select_workspace_size", "ttn_select_f16", "ttn_select_f16_static",
     "ttn_route_experts", "ttn_token_logprobs", "ttn_expert_mlp_workspace_size", "ttn_expert_mlp",
-    "ttn_expert_mlp_fault",
+    "ttn_expert_mlp_fault", "ttn_expert_mlp_test_withhold_copies",
 )
 
 
@@ -133,6 +133,7 @@ _SIGNATURES = {
     "ttn_expert_mlp": (ctypes.c_int, [ctypes.c_int, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _P, _I64,
                                       _P, ctypes.c_size_t, _P]),
     "ttn_expert_mlp_fault": (ctypes.c_int, [ctypes.POINTER(ctypes.c_uint32)]),
+    "ttn_expert_mlp_test_withhold_copies": (None, []),
 }
 
 _lib = None

@@ -23,6 +23,7 @@
 //  * expert_combine adds a token's shares in the order of its choices.
 // Every wait is bounded (200 ms); a role that gives up records why in a device word
 // (ttn_expert_mlp_fault) and the pair frees its TMEM and returns.
+#include <atomic>
 #include <type_traits>
 
 #include "rows.cuh"
@@ -170,6 +171,10 @@ __global__ void __launch_bounds__(kDownWarps * 32) expert_rows_down(ExpertArgs a
 
 __device__ uint32_t g_expert_fault;
 
+// Test hook (ttn_expert_mlp_test_withhold_copies): the next call's first product on the
+// tensor cores issues no operand copy.
+std::atomic<bool> g_withhold_next_products{false};
+
 // offsets[e]: pairs of experts below e; order: the pairs, by expert, then by number.  One
 // block an expert, each reading all ids twice (they are few and in L2), 128 a warp and load:
 // no block waits for another.  65,536 ids of 64 experts take 8 us on a B200.
@@ -264,6 +269,7 @@ struct ProductArgs {
   float* scale;     // down: [pair][blocks]
   int experts, top_k, rows, steps, m_tiles, blocks;  // rows: weight rows of the product (inner or hidden)
   int bf16;
+  int withhold;     // test hook: no operand copy, so every other role's first wait runs out
   int wide;         // down: share rows are multiples of 32 bytes
 };
 struct ProductMaps {
@@ -356,14 +362,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
   cluster_barrier();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int count = tiles[a.experts] * a.m_tiles, first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+  const int count = tiles[a.experts] * a.m_tiles;
+  const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
   TileList list = {offsets, tiles, a.m_tiles, 0};
   uint32_t fault = 0;
 
   if (warp == 0) {  // producer, in both CTAs: this CTA's half of the operands that TMA loads
     int s = 0;
     uint32_t phase = 0;
-    for (int t = first; t < count && !fault; t += stride) {
+    for (int t = first; t < count && !fault && !a.withhold; t += stride) {
       int m, row0, rows;
       list.at(t, m, row0, rows);
       const int half = ((rows + 31) & ~31) / 2;  // rows of the N operand in this CTA
@@ -403,7 +410,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
     const int line = (warp - 2 - kEpiWarps) * 4;
     int s = 0;
     uint32_t phase = 0;
-    for (int t = first; t < count && !fault; t += stride) {
+    for (int t = first; t < count && !fault && !a.withhold; t += stride) {
       int m, row0, rows;
       list.at(t, m, row0, rows);
       const int half = ((rows + 31) & ~31) / 2;
@@ -770,6 +777,7 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     p.m_tiles = (rows + tile - 1) / tile;
     p.blocks = (int)s.blocks;
     p.bf16 = bf16;
+    p.withhold = gate_up && g_withhold_next_products.exchange(false);
     p.wide = a.hidden % 16 == 0;
     if (runs * p.m_tiles > INT32_MAX) return fail(TTN_UNSUPPORTED, "%s: more than 2^31 tiles", name);
     TTN_TRY(ensure_dynamic_smem((const void*)kernel, (int)smem));
@@ -859,6 +867,8 @@ ttn_status ttn_expert_mlp(int dtype, const void* x, int64_t x_row_stride, int64_
   return dtype == TTN_F16 ? launch_experts<F16>(name, a, s, workspace, (cudaStream_t)stream)
                           : launch_experts<BF16>(name, a, s, workspace, (cudaStream_t)stream);
 }
+
+void ttn_expert_mlp_test_withhold_copies(void) { g_withhold_next_products.store(true); }
 
 ttn_status ttn_expert_mlp_fault(uint32_t* fault) {
   const char* name = "ttn_expert_mlp_fault";

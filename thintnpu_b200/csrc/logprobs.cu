@@ -291,10 +291,13 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
     // rising logits), a second time into sorted lists, one a warp: once a list is full only what
     // beats its n-th entry gets in.
     uint64_t list = 0, last = 0;
+    float bar = floor_value;  // elements below it are passed over
+    bool full = false;        // and, once the list is full, those equal to it: they come later
     for (bool sorted = false;; sorted = true) {
       for (int i0 = 0; i0 < own; i0 += 32) {
         const int i = i0 + lane;
-        uint32_t open = __ballot_sync(kAll, i < own && !(seg_top[min(i, own - 1) * kLpWarps + warp] < floor_value));
+        const float t = i < own ? seg_top[i * kLpWarps + warp] : ninf;
+        uint32_t open = __ballot_sync(kAll, t != ninf && !(t < bar));
         while (open) {  // two segments' loads in flight
           const int s0 = seg0 + (i0 + __ffs(open) - 1) * kLpWarps + warp;
           open &= open - 1;
@@ -316,7 +319,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
               T::unpack(v[u][g], f);
 #pragma unroll
               for (int q = 0; q < kVec; ++q)
-                reach |= (uint32_t)(!(f[q] < floor_value)) << ((u * kLpGroup + g) * kVec + q);
+                reach |= (uint32_t)(f[q] != ninf && !(f[q] < bar) && !(full && f[q] == bar))
+                         << ((u * kLpGroup + g) * kVec + q);
             }
           if (!two) reach &= (1u << (kLpGroup * kVec)) - 1;
           while (__any_sync(kAll, reach)) {  // few: each element is read once more by itself
@@ -336,8 +340,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
             } else if (__any_sync(kAll, e > last)) {
               list = merge32(list, sort32(e > last ? e : (uint64_t)0, lane), lane);
               last = __shfl_sync(kAll, list, a.top - 1);
+              full = last != 0;
+              if (full) bar = key_value((uint32_t)(last >> 32));
             }
           }
+          if (!sorted && __any_sync(kAll, *static_cast<volatile int*>(&held) > kLpHeld)) open = 0, i0 = own;  // too many
         }
       }
       __syncthreads();
@@ -411,6 +418,7 @@ ttn_status launch_logprobs(const char* name, LpArgs a, cudaStream_t stream) {
   while (ranks < kLpMaxRanks && a.rows * ranks * 2 <= 2 * sm_count() && segments > ranks * kLpWarps * 2) ranks *= 2;
   a.slice = (segments + ranks - 1) / ranks;
   const size_t smem = a.top ? (size_t)a.slice * 4 : 0;
+  TTN_TRY(ensure_dynamic_smem((const void*)token_logprobs<T>, (int)smem));
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)(a.rows * ranks));
   config.blockDim = dim3(kLpThreads);
