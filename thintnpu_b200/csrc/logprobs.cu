@@ -25,6 +25,7 @@
 // to stay below the 11 issue slots a 16-bit logit at copy speed.
 #include <cooperative_groups.h>
 
+#include <cfloat>
 #include <type_traits>
 
 #include "rows.cuh"
@@ -291,13 +292,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
     // rising logits), a second time into sorted lists, one a warp: once a list is full only what
     // beats its n-th entry gets in.
     uint64_t list = 0, last = 0;
-    float bar = floor_value;  // elements below it are passed over
-    bool full = false;        // and, once the list is full, those equal to it: they come later
+    // Elements below the bar are passed over: masked ones, and once a list is full those equal
+    // to its n-th entry too, as they come later.
+    float bar = floor_value == ninf ? -FLT_MAX : floor_value;
     for (bool sorted = false;; sorted = true) {
       for (int i0 = 0; i0 < own; i0 += 32) {
         const int i = i0 + lane;
         const float t = i < own ? seg_top[i * kLpWarps + warp] : ninf;
-        uint32_t open = __ballot_sync(kAll, t != ninf && !(t < bar));
+        uint32_t open = __ballot_sync(kAll, !(t < bar));
         while (open) {  // two segments' loads in flight
           const int s0 = seg0 + (i0 + __ffs(open) - 1) * kLpWarps + warp;
           open &= open - 1;
@@ -319,8 +321,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
               T::unpack(v[u][g], f);
 #pragma unroll
               for (int q = 0; q < kVec; ++q)
-                reach |= (uint32_t)(f[q] != ninf && !(f[q] < bar) && !(full && f[q] == bar))
-                         << ((u * kLpGroup + g) * kVec + q);
+                reach |= (uint32_t)(!(f[q] < bar)) << ((u * kLpGroup + g) * kVec + q);
             }
           if (!two) reach &= (1u << (kLpGroup * kVec)) - 1;
           while (__any_sync(kAll, reach)) {  // few: each element is read once more by itself
@@ -340,8 +341,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
             } else if (__any_sync(kAll, e > last)) {
               list = merge32(list, sort32(e > last ? e : (uint64_t)0, lane), lane);
               last = __shfl_sync(kAll, list, a.top - 1);
-              full = last != 0;
-              if (full) bar = key_value((uint32_t)(last >> 32));
+              if (last) bar = key_value((uint32_t)(last >> 32) + 1);  // the next value up
             }
           }
           if (!sorted && __any_sync(kAll, *static_cast<volatile int*>(&held) > kLpHeld)) open = 0, i0 = own;  // too many
