@@ -586,7 +586,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float lo = __uint_as_float(v[2 * i]), hi = __uint_as_float(v[2 * i + 1]);
-              w[i] = __byte_perm(__float2int_rn(lo * inverse), __float2int_rn(hi * inverse), 0x5410);
+              // adding 1.5 * 2^23 rounds to an integer and leaves it in the low bits
+              w[i] = __byte_perm(__float_as_uint(fmaf(lo, inverse, 12582912.0f)),
+                                 __float_as_uint(fmaf(hi, inverse, 12582912.0f)), 0x5410);
             }
             if (!whole) {  // zeros, vanishing values, infinities, NaN: as bf16
 #pragma unroll
@@ -627,7 +629,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
 // out[token] = sum of weight * share over the token's choices, in their order; 8 features a thread.
 constexpr int kCombineThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(kCombineThreads) expert_combine(ExpertArgs a, const int16_t* __restrict__ share,
+__global__ void __launch_bounds__(kCombineThreads, 4) expert_combine(ExpertArgs a, const int16_t* __restrict__ share,
                                                                   const float* __restrict__ scale, int blocks,
                                                                   FastDiv groups) {
   pdl_trigger();
@@ -635,43 +637,57 @@ __global__ void __launch_bounds__(kCombineThreads) expert_combine(ExpertArgs a, 
   const uint32_t i = blockIdx.x * kCombineThreads + threadIdx.x;
   const uint32_t token = groups.div(i), f = (i - token * groups.d) * 8;
   if (token >= a.tokens) return;
-  float sum[8] = {};
-  constexpr int kBatch = 8;  // choices whose loads are in flight together
+  unsigned long long sum[4] = {};  // pairs of features (packed arithmetic)
+  constexpr int kBatch = 8;        // choices whose loads are in flight together
   for (int j0 = 0; j0 < a.top_k; j0 += kBatch) {
     const int64_t pair0 = (int64_t)token * a.top_k + j0;
+    const int32_t* ids = a.ids + pair0;
+    const float* weights = a.weights + pair0;
+    const int16_t* from = share + pair0 * a.hidden + f;
+    const float* scales = scale + pair0 * blocks + f / kShareBlock;
     float w[kBatch], sc[kBatch];
     uint4 v[kBatch];
-    bool live[kBatch];
+    uint32_t live = 0;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {  // shares of pairs without an expert were never written
-      live[j] = j0 + j < a.top_k && (unsigned)a.ids[pair0 + j] < (unsigned)a.experts;
-      w[j] = live[j] ? a.weights[pair0 + j] : 0.0f;
-      sc[j] = live[j] ? scale[(pair0 + j) * blocks + f / kShareBlock] : 0.0f;
-      v[j] = live[j] ? *reinterpret_cast<const uint4*>(share + (pair0 + j) * a.hidden + f) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < kBatch; ++j)  // shares of pairs without an expert were never written
+      if (j0 + j < a.top_k && (unsigned)ids[j] < (unsigned)a.experts) live |= 1u << j;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (!(live >> j & 1u)) continue;
+      v[j] = __ldcs(reinterpret_cast<const uint4*>(from + (int64_t)j * a.hidden));
+      w[j] = weights[j];
+      sc[j] = scales[(int64_t)j * blocks];
     }
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      if (!live[j]) continue;
+      if (!(live >> j & 1u)) continue;
       const uint32_t words[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-      if (sc[j] >= 0.0f) {
-        const float ws = w[j] * sc[j];
+      const bool whole = sc[j] >= 0.0f;
+      const float by = whole ? w[j] * sc[j] : w[j];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          sum[2 * q] = fmaf(ws, (float)(int16_t)words[q], sum[2 * q]);
-          sum[2 * q + 1] = fmaf(ws, (float)((int32_t)words[q] >> 16), sum[2 * q + 1]);
+      for (int q = 0; q < 4; ++q) {
+        unsigned long long p;
+        if (whole) {
+          // i -> the FP32 of bits 0x4b000000 + (i + 2^15), which is 2^23 + 2^15 + i
+          const uint32_t u = words[q] ^ 0x80008000u;
+          p = f2_add(f2_pack(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7610)),
+                             __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7632))),
+                     f2_pack(-8421376.0f, -8421376.0f));
+        } else {
+          const float2 b = BF16::two(words[q]);
+          p = f2_pack(b.x, b.y);
         }
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float2 p = BF16::two(words[q]);
-          sum[2 * q] = fmaf(w[j], p.x, sum[2 * q]);
-          sum[2 * q + 1] = fmaf(w[j], p.y, sum[2 * q + 1]);
-        }
+        sum[q] = f2_fma(p, f2_pack(by, by), sum[q]);
       }
     }
   }
-  *reinterpret_cast<uint4*>(a.out + token * a.out_stride + f) =
-      make_uint4(T::round2(sum[0], sum[1]), T::round2(sum[2], sum[3]), T::round2(sum[4], sum[5]), T::round2(sum[6], sum[7]));
+  uint32_t out[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float2 p = f2_unpack(sum[q]);
+    out[q] = T::round2(p.x, p.y);
+  }
+  *reinterpret_cast<uint4*>(a.out + token * a.out_stride + f) = make_uint4(out[0], out[1], out[2], out[3]);
 }
 
 // Up to this many pairs each pair reads its expert's weights by itself.  64 experts, hidden
