@@ -557,7 +557,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
         } else {
           // 16 columns at a time through shared memory: two lanes a row then hold 16 neighbouring
           // features each, so the row's largest is found in registers (a warp-wide reduction a
-          // column made this epilogue 200 cycles a column and the product 434 us, now 215 us).
+          // column made this epilogue 200 cycles a column and the product 434 us, now 258 us).
           const int f0 = tile * 256 + (int)rank * 128 + quarter * 32;
           const int n = lane >> 1, f = f0 + (lane & 1) * 16;
           uint32_t* in = reinterpret_cast<uint32_t*>(own) + lane;

@@ -9,6 +9,8 @@ RuntimeError, never fall back to another implementation.
 from __future__ import annotations
 
 import ctypes
+import struct
+import threading
 from typing import Optional, Sequence
 
 import torch
@@ -631,15 +633,33 @@ def _inputs(what: str, *tensors) -> None:
             _cuda(t, what)
 
 
+_ROWS_LAYOUT = struct.Struct(f"@Pii2q{8 * (_lib.MAX_DIMS - 2)}x2q")  # a two-dim TtnTensor
+
+
+class _RowsDescriptor(threading.local):
+    """A TtnTensor of the calling thread, rewritten by each call (building one anew costs a
+    call a microsecond more)."""
+
+    def __init__(self):
+        self.buffer = bytearray(ctypes.sizeof(TtnTensor))
+        self.tensor = TtnTensor.from_buffer(self.buffer)
+
+
+_rows_descriptor = _RowsDescriptor()
+
+
 def _score_rows(x: torch.Tensor, what: str) -> TtnTensor:
-    """Descriptor of a [rows, columns] view of f16, bf16 or f32 scores."""
+    """Descriptor of a [rows, columns] view of f16, bf16 or f32 scores, valid until the
+    thread's next."""
     _inputs(what, x)
     dtype = _ROW_DTYPES.get(x.dtype)
     if x.dim() != 2:
         _fail(f"{what}: logits must be [rows, columns]")
     if dtype is None:
         _fail(f"{what}: unsupported dtype {x.dtype}: float16/bfloat16/float32 only")
-    return TtnTensor(x.data_ptr(), 2, dtype, tuple(x.shape), x.stride())
+    d = _rows_descriptor
+    _ROWS_LAYOUT.pack_into(d.buffer, 0, x.data_ptr(), 2, dtype, *x.shape, *x.stride())
+    return d.tensor
 
 
 def _like_output(t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device, what: str) -> None:
