@@ -376,7 +376,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
       const int half = ((rows + 31) & ~31) / 2;  // rows of the N operand in this CTA
       for (int step = 0; step < a.steps; ++step) {
         // a fresh barrier counts as freed; the vote keeps the lanes within one step of each other
-        if (!__all_sync(kAll, mbar_wait_cluster<true>(empty_bar(s), phase ^ 1))) {
+        if (!__all_sync(kAll, mbar_wait_cluster(empty_bar(s), phase ^ 1))) {
           fault = 2;
           break;
         }
@@ -421,7 +421,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
         from[i / 4][i % 4] = a.order[row0 + min(row, rows - 1)] / a.top_k;
       }
       for (int step = 0; step < a.steps; ++step) {
-        if (!__all_sync(kAll, mbar_wait_cluster<true>(empty_bar(s), phase ^ 1))) {
+        if (!__all_sync(kAll, mbar_wait_cluster(empty_bar(s), phase ^ 1))) {
           fault = 2;
           break;
         }
@@ -450,7 +450,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
         // kSubs 1: accumulator j & 1, filled every second tile; 2: accumulator u of sub-tile u, every tile
         const int acc = kSubs == 1 ? j & 1 : 0;
         const uint32_t turn = (uint32_t)(kSubs == 1 ? j >> 1 : j) & 1;
-        if (!__all_sync(kAll, mbar_wait_cluster<true>(acc_empty(acc), turn ^ 1))) {
+        if (!__all_sync(kAll, mbar_wait_cluster(acc_empty(acc), turn ^ 1))) {
           fault = 4;
           break;
         }
@@ -466,7 +466,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
         int held = 0;        // kSubs 2: stages up to this one that sub-tile 1 has not taken yet
         bool open = false;   // and whether its accumulator is free
         for (int step = 0; step < a.steps; ++step) {
-          if (!__all_sync(kAll, mbar_wait_cluster<true>(full_bar(s), phase))) {
+          if (!__all_sync(kAll, mbar_wait_cluster(full_bar(s), phase))) {
             fault = 1;
             break;
           }
@@ -487,7 +487,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
             ++held;
             if (!open) {
               const bool must = last || held == kStages;  // nothing more can be loaded before
-              open = __all_sync(kAll, must ? mbar_wait_cluster<true>(acc_empty(1), turn ^ 1)
+              open = __all_sync(kAll, must ? mbar_wait_cluster(acc_empty(1), turn ^ 1)
                                            : mbar_test_cluster(acc_empty(1), turn ^ 1));
               if (must && !open) {
                 fault = 4;
@@ -525,7 +525,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
 #pragma unroll 1
       for (int u = 0; u < kSubs; ++u) {
         const int acc = kSubs == 1 ? j & 1 : u, tile = m * kSubs + u;
-        if (!__all_sync(kAll, mbar_wait_cluster<false>(acc_full(acc), (uint32_t)(kSubs == 1 ? j >> 1 : j) & 1))) {
+        if (!__all_sync(kAll, mbar_wait_cluster(acc_full(acc), (uint32_t)(kSubs == 1 ? j >> 1 : j) & 1))) {
           fault = 4;
           break;
         }

@@ -190,30 +190,20 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) 
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_mbar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_mbar) : "memory");
 }
-// mbar_wait for a barrier that the other CTA of the pair signals too.  kPoll: test_wait, which
-// does not suspend the thread, for the roles that every stage waits for.  The wall clock is
-// read only once a wait has failed a number of times: in a running pipeline most do not.
-template <bool kPoll>
+// mbar_wait for a barrier that the other CTA of the pair signals too.  The wall clock is read
+// only once a wait has failed a number of times: in a running pipeline most do not.
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t mbar, uint32_t phase) {
   uint64_t start = 0;
   for (uint32_t tries = 1;; ++tries) {
     uint32_t done;
-    if (kPoll)
-      asm volatile(
-          "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-          "selp.b32 %0, 1, 0, p;\n\t}\n"
-          : "=r"(done)
-          : "r"(mbar), "r"(phase)
-          : "memory");
-    else
-      asm volatile(
-          "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-          "selp.b32 %0, 1, 0, p;\n\t}\n"
-          : "=r"(done)
-          : "r"(mbar), "r"(phase)
-          : "memory");
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(mbar), "r"(phase)
+        : "memory");
     if (done) return true;
-    if ((tries & (kPoll ? 255u : 15u)) == 0u) {
+    if ((tries & 15u) == 0u) {
       const uint64_t now = global_ns();
       if (!start) start = now;
       if (now - start > kWaitNs) return false;
