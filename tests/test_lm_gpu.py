@@ -176,6 +176,9 @@ MLP = [  # tokens, hidden, inner, experts, top_k, dropped, skew
     (2, 1032, 688, 4, 2, 0.0, 0.0), (17, 72, 16, 7, 1, 0.0, 0.0), (40, 264, 112, 6, 4, 0.25, 0.0),
     (129, 64, 64, 3, 2, 0.0, 0.5), (300, 128, 144, 2, 2, 0.1, 0.0), (65, 520, 272, 40, 6, 0.0, 0.05),
     (600, 40, 32, 4, 3, 0.0, 1.0), (33, 512, 256, 2, 1, 0.0, 3.0), (260, 328, 208, 1, 1, 0.0, 0.0),
+    # more than 256 pairs: on the tensor cores, down to the smallest sizes
+    (300, 8, 16, 1, 1, 0.0, 0.0), (280, 1032, 688, 4, 2, 0.1, 0.0), (90, 264, 112, 6, 4, 0.25, 0.0),
+    (257, 64, 48, 64, 1, 0.0, 0.0), (34, 512, 256, 3, 1, 0.0, 0.0), (20, 2048, 1024, 3, 1, 0.0, 0.0),
     # many rows an expert: two sub-tiles in the first product, in the second, in both with ragged runs
     (2400, 72, 2048, 2, 2, 0.0, 0.3), (4760, 2048, 48, 3, 2, 0.1, 0.4), (5000, 1000, 992, 5, 2, 0.05, 0.2)]
 
@@ -188,7 +191,7 @@ def test_mlp_sizes(device, dtype, tokens, hidden, inner, experts, top_k, dropped
     check_mlp(ttn.expert_mlp(*(t.to(device) for t in args)), args)
 
 
-@pytest.mark.parametrize("tokens", [2, 90])
+@pytest.mark.parametrize("tokens", [2, 90, 200])
 def test_mlp_strided_rows_and_output(device, tokens):
     import thintnpu_b200 as ttn
     args = mlp_inputs(tokens, 96, 32, 4, 2, torch.bfloat16, 5)

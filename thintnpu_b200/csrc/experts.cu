@@ -1,8 +1,8 @@
 // Gated products of the chosen experts:
 //   out[t] = sum_j w[t][j] down[e] (silu(gate[e] x[t]) * (up[e] x[t])),  e = experts[t][j].
 //
-// Few pairs (token, choice): the experts' weights are read once for each pair by
-// ordinary warps, two launches in all (expert_rows_gate_up, expert_rows_down).
+// Few pairs (token, choice; few_pairs says how few): the experts' weights are read once for
+// each pair by ordinary warps, two launches in all (expert_rows_gate_up, expert_rows_down).
 //
 // More pairs: the tensor cores, four launches.
 //  * expert_plan sorts the pairs by expert (stable): offsets[E + 1], order[pairs].
@@ -690,10 +690,17 @@ __global__ void __launch_bounds__(kCombineThreads, 4) expert_combine(ExpertArgs 
   *reinterpret_cast<uint4*>(a.out + token * a.out_stride + f) = make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-// Up to this many pairs each pair reads its expert's weights by itself.  64 experts, hidden
-// 2048, inner 1024, 8 choices: 32 pairs 63 us (on the tensor cores 73), 48 pairs 87 (80); 10
-// experts, hidden 1032, inner 688, 2 choices: 16 pairs 14 us (22), 32 pairs 23.3 (23.7).
-constexpr int64_t kRowsPairs = 32;
+// Whether each pair reads its expert's weights by itself, on ordinary warps: where all those
+// readings are few bytes, or few pairs meet many experts, so that they read most of them once.
+// The tensor cores' four dependent launches take 15 us and more.  Both sides measured (rows /
+// tensor cores, us; bf16): hidden 256, inner 128, 8 experts: 128 pairs 8.7 / 15.1, 256 pairs 14.5 /
+// 15.6, 512 pairs 26 / 17; 512, 256, 16: 128 pairs (101 MB) 16.1 / 16.8; 1024, 512, 32: 40 pairs
+// (126 MB) 24 / 32, 64 pairs 32 / 33, 128 pairs 51 / 33; 2048, 1024, 8: 20 pairs (252 MB) 34 / 29;
+// 2048, 1024, 64: 32 pairs (403 MB) 63 / 73, 48 pairs 87 / 80.
+bool few_pairs(int64_t pairs, int64_t hidden, int64_t inner, int64_t experts) {
+  const int64_t bytes = 6 * hidden * inner;  // of one expert's weights
+  return (pairs <= 256 && pairs * bytes <= 128 * 1000 * 1000) || (pairs <= 32 && 2 * pairs <= experts);
+}
 
 // Whether the first product takes two sub-tiles: experts with many rows, no more padding of
 // the weight rows, and tiles enough for every pair of SMs.  64 experts, hidden 2048, inner 1024,
@@ -719,7 +726,7 @@ bool sizes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64
   auto pad = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
   s->pairs = tokens * top_k;
   s->blocks = (hidden + kShareBlock - 1) / kShareBlock;
-  s->rows = s->pairs <= kRowsPairs;
+  s->rows = few_pairs(s->pairs, hidden, inner, experts);
   if (s->rows) {
     s->order = s->h = s->share = s->scale = 0;
     s->total = pad(s->pairs * inner * 4);

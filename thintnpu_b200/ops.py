@@ -648,18 +648,22 @@ class _RowsDescriptor(threading.local):
 _rows_descriptor = _RowsDescriptor()
 
 
-def _score_rows(x: torch.Tensor, what: str) -> TtnTensor:
-    """Descriptor of a [rows, columns] view of f16, bf16 or f32 scores, valid until the
-    thread's next."""
+def _check_rows(x: torch.Tensor, what: str) -> int:
+    """The dtype code of a [rows, columns] view of f16, bf16 or f32 scores."""
     _inputs(what, x)
     dtype = _ROW_DTYPES.get(x.dtype)
     if x.dim() != 2:
         _fail(f"{what}: logits must be [rows, columns]")
     if dtype is None:
         _fail(f"{what}: unsupported dtype {x.dtype}: float16/bfloat16/float32 only")
+    return dtype
+
+
+def _rows(x: torch.Tensor, dtype: int):
+    """Reference to the thread's descriptor of x, for the next library call."""
     d = _rows_descriptor
     _ROWS_LAYOUT.pack_into(d.buffer, 0, x.data_ptr(), 2, dtype, *x.shape, *x.stride())
-    return d.tensor
+    return ctypes.byref(d.tensor)
 
 
 def _like_output(t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device, what: str) -> None:
@@ -683,7 +687,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     for which no expert is left hold id -1 and weight 0.  ``out`` is a (weights, experts)
     pair to fill."""
     what = "route_experts"
-    d = _score_rows(logits, what)
+    dtype = _check_rows(logits, what)
     if score not in ("softmax", "sigmoid"):
         _fail(f"{what}: score must be 'softmax' or 'sigmoid'")
     rows, experts = logits.shape
@@ -704,7 +708,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
         _like_output(weights, (rows, top_k), torch.float32, device, "route_experts: out weights")
         _like_output(ids, (rows, top_k), torch.int32, device, "route_experts: out experts")
     flags = (_lib.ROUTE_SIGMOID if score == "sigmoid" else 0) | (_lib.ROUTE_RENORMALIZE if renormalize else 0)
-    _call_on(device, "ttn_route_experts", _ref(d), bias_ptr, top_k, groups,
+    _call_on(device, "ttn_route_experts", _rows(logits, dtype), bias_ptr, top_k, groups,
              groups if top_groups is None else top_groups, group_top, flags, scale, weights.data_ptr(),
              ids.data_ptr())
     return weights, ids
@@ -784,7 +788,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     with nothing left has entropy 0.  A NaN or +inf in a row makes its log probabilities
     and entropy NaN."""
     what = "token_logprobs"
-    d = _score_rows(logits, what)
+    dtype = _check_rows(logits, what)
     rows, device = logits.size(0), logits.device
     _inputs(what, tokens)
     _like_output(tokens, (rows,), torch.int64, device, "token_logprobs: tokens")
@@ -795,6 +799,6 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0, 
     entropy = logits.new_empty(rows, dtype=torch.float32)
     top_logprobs = logits.new_empty((rows, top), dtype=torch.float32)
     top_tokens = logits.new_empty((rows, top), dtype=torch.int32)
-    _call_on(device, "ttn_token_logprobs", _ref(d), tokens.data_ptr(), scale, top, logprobs.data_ptr(),
+    _call_on(device, "ttn_token_logprobs", _rows(logits, dtype), tokens.data_ptr(), scale, top, logprobs.data_ptr(),
              entropy.data_ptr(), top_logprobs.data_ptr() if top else None, top_tokens.data_ptr() if top else None)
     return logprobs, entropy, top_logprobs, top_tokens
