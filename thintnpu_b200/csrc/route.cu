@@ -20,6 +20,8 @@
 // speed), but a few hundred instructions: the kernel is bound by instruction issue.  On a
 // B200 16,384 such rows with a bias and groups take 25 us (62 us when each choice was a
 // warp-wide maximum and close groups took the whole row in 64 bits).
+#include <cfloat>
+
 #include "rows.cuh"
 
 namespace ttn {
@@ -143,7 +145,7 @@ __device__ __noinline__ int route_exact(const RouteArgs& a, int64_t row, float m
 
 // W: room for a lane's experts (>= a.width).
 template <typename T, int W>
-__global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
+__global__ void __launch_bounds__(kRouteThreads, W <= 8 ? 12 : 4) route_rows(RouteArgs a) {
   extern __shared__ double shared_ranks[];  // [warps][E]
   __shared__ float2 packed[kRouteWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -345,9 +347,10 @@ __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
         if (best == floor_rank) best = ninf;
       }
       const uint32_t before = (1u << lane) - 1;
+      const float bar = fmaxf(floor_rank, -FLT_MAX);
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        const bool in = v[i] >= floor_rank && v[i] != ninf;
+        const bool in = v[i] >= bar;
         const uint32_t vote = __ballot_sync(kAll, in);
         const int at = n + __popc(vote & before);
         if (in && at < 32) packed[warp][at] = make_float2(v[i], __int_as_float(first + i));
@@ -445,13 +448,13 @@ __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
   const float chosen = a.renormalize ? warp_largest(xm) : 0.0f;
   if (mine >= 0) {
     if (a.sigmoid)
-      s = a.renormalize && chosen < -20.0f ? expf(xm - chosen) : 1.0f / (1.0f + expf(-xm));
+      s = a.renormalize && chosen < -20.0f ? expf(xm - chosen) : __fdividef(1.0f, 1.0f + expf(-xm));
     else
       s = poisoned ? m : a.renormalize ? expf(xm - chosen) : expf(xm - m) * inverse;
   }
   if (a.renormalize) {
     const float sum = warp_sum(s);
-    s = sum == 0.0f ? 0.0f : s / sum;
+    s = sum == 0.0f ? 0.0f : __fdividef(s, sum);
   }
   if (lane < a.top_k) {
     a.weights[row * a.top_k + lane] = mine >= 0 ? s * a.scale : 0.0f;
