@@ -4,8 +4,9 @@
 // Few pairs (token, choice; few_pairs says how few): the experts' weights are read once for
 // each pair by ordinary warps, two launches in all (expert_rows_gate_up, expert_rows_down).
 //
-// More pairs: the tensor cores, four launches.
-//  * expert_plan sorts the pairs by expert (stable): offsets[E + 1], order[pairs].
+// More pairs: the tensor cores, three or four launches.
+//  * expert_plan sorts the pairs by expert (stable): offsets[E + 1], order[pairs].  A few
+//    pairs are sorted by each block of the first product instead.
 //  * expert_products<gate-up> and <down>: grouped matrix products on pairs of CTAs
 //    (tcgen05, cta_group::2), persistent and warp-specialised.  The weights are the M
 //    operand (128 rows a CTA) and an expert's rows the N operand (32 to 256 in steps of
@@ -263,7 +264,9 @@ constexpr uint32_t staging_bytes(bool gate_up) { return gate_up ? 32 * 16 * 2 : 
 constexpr int kShareBlock = 32;              // features that share a scale
 
 struct ProductArgs {
-  const int32_t *offsets, *order;
+  int32_t *offsets, *order;
+  const int32_t* ids;  // gate-up: sort these pairs here (block 0 leaves the result); null: they are sorted
+  int pairs;
   uint16_t* h;      // gate-up: [pairs, sorted][inner]
   int16_t* share;   // down: [pair][hidden], integers (or bf16 where the scale is negative)
   float* scale;     // down: [pair][blocks]
@@ -272,11 +275,17 @@ struct ProductArgs {
   int withhold;     // test hook: no operand copy, so every other role's first wait runs out
   int wide;         // down: share rows are multiples of 32 bytes
 };
+// Up to this many pairs every block of the first product sorts them for itself instead of a
+// launch of expert_plan (3 us of the host's time a call).  With the launch / without, us: 512
+// pairs of 8 experts (hidden 256, inner 128) 17.7 / 16.6, 320 of 64 (1024, 512) 55.9 / 54.1, 1024
+// of 32 (1024, 512) 37.0 / 37.2, 2048 of 32 41.4 / 42.8.
+constexpr int kSortHere = 1024;
 struct ProductMaps {
   CUtensorMap a, b;
 };
 __host__ __device__ constexpr uint32_t product_smem(bool gate_up, int experts) {
-  return 1024 + kRingBytes + epi_warps(gate_up) * staging_bytes(gate_up) + 2 * 4 * (uint32_t)(experts + 1);
+  return 1024 + kRingBytes + epi_warps(gate_up) * staging_bytes(gate_up) + (gate_up ? kSortHere * 4 : 0) +
+         2 * 4 * (uint32_t)(experts + 1);
 }
 
 // Tile t of the list: experts in order, of an expert its runs of rows, of a run its weight rows.
@@ -295,6 +304,61 @@ struct TileList {
     count = min(n, all - i * n);
   }
 };
+
+// expert_plan's result for a few pairs, by all threads of a block: offsets[E + 1] and order in
+// shared memory.  counts: [warps][E], room that is free for now.  Each warp counts the experts
+// of its run of pairs, the runs' counts become their places, and the pairs go to them in order.
+__device__ __forceinline__ void sort_pairs(const int32_t* __restrict__ ids, int pairs, int experts, int32_t* counts,
+                                           int32_t* offsets, int32_t* order) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int chunk = (pairs + warps * 32 - 1) / (warps * 32) * 32;
+  const int first = warp * chunk, last = min(first + chunk, pairs);
+  int32_t* mine = counts + warp * experts;
+  for (int e = lane; e < experts; e += 32) mine[e] = 0;
+  __syncwarp();
+  auto pass = [&](bool place) {
+    for (int i0 = first; i0 < last; i0 += 32) {
+      const int id = i0 + lane < last ? __ldg(ids + i0 + lane) : -1;
+      const bool valid = (unsigned)id < (unsigned)experts;
+      const uint32_t same = __match_any_sync(kAll, valid ? id : -1);
+      const int before = __popc(same & ((1u << lane) - 1));
+      if (place && valid) order[offsets[id] + mine[id] + before] = i0 + lane;
+      __syncwarp();
+      if (valid && !before) mine[id] += __popc(same);
+      __syncwarp();
+    }
+  };
+  pass(false);
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+    int sum = 0;
+    for (int w = 0; w < warps; ++w) {
+      const int n = counts[w * experts + e];
+      counts[w * experts + e] = sum;
+      sum += n;
+    }
+    offsets[e] = sum;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int sum = 0;
+    for (int base = 0; base < experts; base += 32) {
+      const int n = base + lane < experts ? offsets[base + lane] : 0;
+      int to = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(kAll, to, d);
+        if (lane >= d) to += v;
+      }
+      if (base + lane < experts) offsets[base + lane] = sum + to - n;
+      sum += __shfl_sync(kAll, to, 31);
+    }
+    if (lane == 0) offsets[experts] = sum;
+  }
+  __syncthreads();
+  pass(true);
+  __syncthreads();
+}
 
 // kGateUp: the first product, whose token rows are gathered from x through `order`.
 // kSubs: weight-row tiles of 256 that share each stage's token rows.  1: two accumulators, so
@@ -318,7 +382,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
   const uint32_t smem0 = ((uint32_t)__cvta_generic_to_shared(smem) + 1023u) & ~1023u;
   unsigned char* generic0 = smem + (smem0 - (uint32_t)__cvta_generic_to_shared(smem));
   unsigned char* staging = generic0 + kRingBytes;
-  int32_t* offsets = reinterpret_cast<int32_t*>(staging + kEpiWarps * staging_bytes(kGateUp));
+  int32_t* sorted = reinterpret_cast<int32_t*>(staging + kEpiWarps * staging_bytes(kGateUp));
+  int32_t* offsets = sorted + (kGateUp ? kSortHere : 0);
   int32_t* tiles = offsets + a.experts + 1;
   const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(&bars[0]);
   auto full_bar = [&](int s) { return bar0 + 8 * s; };
@@ -340,11 +405,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
   }
   if (warp == 1) tmem_pair_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), 2 * kTileN);
   pdl_wait();
+  const bool here = kGateUp && a.ids;
+  if (here) {  // (the ring is free: no copy has been issued)
+    sort_pairs(a.ids, a.pairs, a.experts, reinterpret_cast<int32_t*>(generic0), offsets, sorted);
+    fence_proxy_async_smem();
+    if (blockIdx.x == 0) {  // for the second product
+      for (int i = tid; i <= a.experts; i += blockDim.x) a.offsets[i] = offsets[i];
+      for (int i = tid; i < offsets[a.experts]; i += blockDim.x) a.order[i] = sorted[i];
+    }
+  }
+  const int32_t* order = here ? sorted : a.order;
   if (warp == 0) {  // the list of tiles: runs of at most kTileN rows of each expert
+    const int32_t* from = here ? offsets : a.offsets;
     int sum = 0;
     for (int base = 0; base < a.experts; base += 32) {
       const int e = base + lane;
-      const int o = e <= a.experts ? a.offsets[e] : 0, next = e < a.experts ? a.offsets[e + 1] : o;
+      const int o = e <= a.experts ? from[e] : 0, next = e < a.experts ? from[e + 1] : o;
       int runs = (next - o + kTileN - 1) / kTileN;
       const int own = runs;
 #pragma unroll
@@ -352,10 +428,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
         const int v = __shfl_up_sync(kAll, runs, d);
         if (lane >= d) runs += v;
       }
-      if (e < a.experts) offsets[e] = o, tiles[e] = sum + runs - own;
+      if (e < a.experts) tiles[e] = sum + runs - own;
+      if (!here && e < a.experts) offsets[e] = o;
       sum += __shfl_sync(kAll, runs, 31);
     }
-    if (lane == 0) offsets[a.experts] = a.offsets[a.experts], tiles[a.experts] = sum;
+    if (lane == 0) tiles[a.experts] = sum;
+    if (!here && lane == 0) offsets[a.experts] = from[a.experts];
   }
   tc_fence_before();
   __syncthreads();
@@ -418,7 +496,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
 #pragma unroll
       for (int i = 0; i < kGatherRows; ++i) {  // past the run's end: its last row (those columns are not stored)
         const int row = (int)rank * half + line + i / 4 * (4 * kGatherWarps) + i % 4;
-        from[i / 4][i % 4] = a.order[row0 + min(row, rows - 1)] / a.top_k;
+        from[i / 4][i % 4] = order[row0 + min(row, rows - 1)] / a.top_k;
       }
       for (int step = 0; step < a.steps; ++step) {
         if (!__all_sync(kAll, mbar_wait_cluster(empty_bar(s), phase ^ 1))) {
@@ -563,7 +641,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
           uint32_t* in = reinterpret_cast<uint32_t*>(own) + lane;
           const uint4* back = reinterpret_cast<const uint4*>(own) + (n * kStagingPitch + (lane & 1) * 16) / 4;
           for (int c = group * 16; c < rows && f0 < a.rows; c += kEpiGroups * 16) {
-            const int pair = c + n < rows ? a.order[row0 + c + n] : -1;
+            const int pair = c + n < rows ? order[row0 + c + n] : -1;
             uint32_t r[16];
             tmem_ld16(lanes + acc * kTileN + c, r);
 #pragma unroll
@@ -786,7 +864,9 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     const cuuint32_t box[2] = {kStepK, 16};
     TTN_TRY(encode_map(name, &down.b, bf16, 2, h, dims, str, box));
   }
-  TTN_TRY(cuda_check(launch_pdl(expert_plan, dim3((unsigned)a.experts), dim3(kPlanThreads), 0, stream, a.ids,
+  const bool here = s.pairs <= kSortHere;
+  if (!here)
+    TTN_TRY(cuda_check(launch_pdl(expert_plan, dim3((unsigned)a.experts), dim3(kPlanThreads), 0, stream, a.ids,
                                 (int)s.pairs, a.experts, (int)((uintptr_t)a.ids % 16 == 0), offsets, order),
                      name));
   const int64_t runs = s.pairs / kTileN + (s.pairs < a.experts ? s.pairs : a.experts);  // at most
@@ -795,6 +875,7 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     const uint32_t smem = product_smem(gate_up, a.experts);
     ProductArgs p = {};
     p.offsets = offsets, p.order = order, p.h = h, p.share = share, p.scale = scale;
+    p.ids = here && gate_up ? a.ids : nullptr, p.pairs = (int)s.pairs;
     p.experts = a.experts, p.top_k = a.top_k, p.rows = rows;
     p.steps = (length + kStepK - 1) / kStepK;
     p.m_tiles = (rows + tile - 1) / tile;
