@@ -12,5 +12,7 @@ golden outputs of the reference's own CPU restatement (``reference()`` in
 verify_selection_flow.py) on its 47 fixtures and the exhaustive 65,536-half
 key/float-bits checks; the elementwise/layout oracles are the reference
 tests' own CPU formulas (verify_flow_ops.py:13-35, verify_softmax.py,
-verify_dfl_softmax.py, verify_ops.py, verify_all.py).
+verify_dfl_softmax.py, verify_ops.py, verify_all.py).  ``oracle.lm`` restates the
+language-model operators in 64 bits; ``tests/test_lm_oracle.py`` checks it against
+PyTorch's own softmax, topk and log_softmax.
 """

@@ -2,7 +2,8 @@
 
 ``libttn.so`` (include/ttn.h) is the product: hand-written kernels behind a
 C ABI.  This package binds it with ctypes and exposes the reference's
-``thin_backend`` operator surface on CUDA tensors.  The library loads on the
+``thin_backend`` operator surface on CUDA tensors, with the serving operators of a
+mixture-of-experts language model beside it.  The library loads on the
 first op call (or ``load()``) and a missing library raises ImportError -- there
 is no CPU or PyTorch fallback.
 """
