@@ -11,7 +11,7 @@
 //
 // The order is the mathematical one, not that of rounded scores.  softmax and sigmoid
 // rise with x, so without a bias the rank is x itself.  With a bias (or a group's sum of
-// two scores) ranks are fp32 sums with an error below kBand; neighbours in the chosen
+// two scores) ranks are fp32 sums with an error below rank_band; neighbours in the chosen
 // order that lie closer than that are ranked again in 64 bits, one candidate a lane, and so
 // are the groups' best where the last group kept and the first left out are that close.  On
 // N(0, 1.5) logits with 256 experts about one row in two hundred has such neighbours.
@@ -31,11 +31,16 @@ constexpr int kRouteThreads = 128;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kMaxTopK = 16;  // leaves 16 lanes for candidates behind the last choice
 constexpr uint32_t kAll = 0xffffffffu;
-// Two fp32 ranks further apart than kBand * max(1, |rank|) are in the order of their exact
-// values: the exp2 and reciprocal approximations (2 ulp each), x - max, the products and the
-// sum's own error leave s within 8 * 2^-24 of its value (s <= 1), the bias addition rounds by |rank| 2^-24 more, twice that
-// for a difference, and a group's sum of two doubles it again: 36 * 2^-24 = 2.2e-6.
-constexpr float kBand = 2.5e-6f;
+// Two fp32 ranks further apart than band * max(1, |rank|) are in the order of their exact
+// values.  With u = 2^-24: a sigmoid score is within 8 u (exp2 and reciprocal approximations
+// of 2 ulp, the argument's rounding, 1 + e); a softmax score within (W + 19) u, as its
+// total of W terms a lane and five shuffles rounds W + 4 times and each term is within 6 u
+// (s |x - m| <= 0.37).  The bias addition rounds by |rank| u more; a difference doubles that
+// and a group's sum of two doubles it again.
+template <int W>
+__device__ __forceinline__ float rank_band(bool sigmoid) {
+  return (sigmoid ? 4.0f * 9.0f : 4.0f * (W + 20.0f)) * 5.9604645e-8f;
+}
 
 struct RouteArgs {
   const void* logits;
@@ -152,7 +157,7 @@ __global__ void __launch_bounds__(kRouteThreads, W <= 8 ? 12 : 4) route_rows(Rou
   const int64_t row = (int64_t)blockIdx.x * kRouteWarps + warp;
   if (row >= a.rows) return;  // whole warps
   const int w = a.width, first = lane * w;
-  const float ninf = -__int_as_float(0x7f800000);
+  const float ninf = -__int_as_float(0x7f800000), band = rank_band<W>(a.sigmoid);
 
   float v[W];  // logits, then ranks; -inf: none
 #pragma unroll
@@ -264,7 +269,7 @@ __global__ void __launch_bounds__(kRouteThreads, W <= 8 ? 12 : 4) route_rows(Rou
       const uint32_t out = __ballot_sync(kAll, lane < a.groups && rank == a.top_groups);
       const float inner = __shfl_sync(kAll, strength, __ffs(in) - 1);
       const float outer = __shfl_sync(kAll, strength, __ffs(out) - 1);
-      if (inner - outer <= kBand * fmaxf(1.0f, fabsf(inner))) {  // not so for infinities
+      if (inner - outer <= band * fmaxf(1.0f, fabsf(inner))) {  // not so for infinities
         // The last group kept and the first left out are too close for fp32: the experts that can
         // be among their group's group_top, one a lane, ranked in 64 bits.
         const float least = a.group_top == 2 && t2 != ninf ? t2 : t1;
@@ -272,7 +277,7 @@ __global__ void __launch_bounds__(kRouteThreads, W <= 8 ? 12 : 4) route_rows(Rou
 #pragma unroll
         for (int i = 0; i < W; ++i) {
           const float bar = __shfl_sync(kAll, least, min(first + i, a.experts - 1) / a.group_size);
-          const bool can = v[i] != ninf && v[i] >= bar - kBand * fmaxf(1.0f, fabsf(bar));
+          const bool can = v[i] != ninf && v[i] >= bar - band * fmaxf(1.0f, fabsf(bar));
           const uint32_t vote = __ballot_sync(kAll, can);
           const int at = n + __popc(vote & ((1u << lane) - 1));
           if (can && at < 32) packed[warp][at].y = __int_as_float(first + i);
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(kRouteThreads, W <= 8 ? 12 : 4) route_rows(Rou
     // close: pairs to be ranked again; run: pairs within the band, equal ones too
     auto neighbours = [&](int n, uint32_t& close, uint32_t& run) {
       const float next = __shfl_down_sync(kAll, val, 1);
-      const bool in_band = lane + 1 < n && val - next <= kBand * fmaxf(1.0f, fabsf(val));
+      const bool in_band = lane + 1 < n && val - next <= band * fmaxf(1.0f, fabsf(val));
       run = __ballot_sync(kAll, in_band);
       close = 0;
       if (!run) return;
