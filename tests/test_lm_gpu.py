@@ -117,6 +117,17 @@ def test_route_close_ranks_are_ordered_exactly(device):
             check_route(device, x, top_k, score=score, bias=bias, groups=4, top_groups=2, group_top=2)
 
 
+def test_route_close_ranks_of_many_experts(device):
+    """1024 softmax scores and biases that undo their differences to a few roundings."""
+    g = torch.Generator().manual_seed(13)
+    x = (torch.randn(1, 1024, generator=g) * 4).repeat(6, 1)
+    s = torch.softmax(x.double(), 1)
+    bias = (0.5 - s[0]).float()
+    bias += torch.randint(-30, 31, (1024,), generator=g) * 2.0 ** -24
+    check_route(device, x, 16, bias=bias)
+    check_route(device, x, 16, bias=bias, groups=32, top_groups=7, group_top=2, renormalize=True)
+
+
 def test_route_small_sigmoids_keep_their_ratios(device):
     logits = torch.tensor([[-90.0, -91.0, -95.0, -130.0], [-19.5, -20.5, -21.0, -200.0]])
     check_route(device, logits, 3, score="sigmoid", renormalize=True)
@@ -179,6 +190,9 @@ MLP = [  # tokens, hidden, inner, experts, top_k, dropped, skew
     # more than 256 pairs: on the tensor cores, down to the smallest sizes
     (300, 8, 16, 1, 1, 0.0, 0.0), (280, 1032, 688, 4, 2, 0.1, 0.0), (90, 264, 112, 6, 4, 0.25, 0.0),
     (257, 64, 48, 64, 1, 0.0, 0.0), (34, 512, 256, 3, 1, 0.0, 0.0), (20, 2048, 1024, 3, 1, 0.0, 0.0),
+    # the most experts and the most choices
+    (400, 16, 16, 1024, 2, 0.0, 0.0), (1200, 24, 32, 1024, 2, 0.1, 0.0), (40, 40, 16, 64, 32, 0.3, 0.0),
+    (1, 64, 32, 40, 32, 0.1, 0.0),
     # many rows an expert: two sub-tiles in the first product, in the second, in both with ragged runs
     (2400, 72, 2048, 2, 2, 0.0, 0.3), (4760, 2048, 48, 3, 2, 0.1, 0.4), (5000, 1000, 992, 5, 2, 0.05, 0.2)]
 
