@@ -410,8 +410,9 @@ ttn_status ttn_select_f16_static(const ttn_tensor* decoded, int64_t max_det, uin
  * with TTN_ROUTE_RENORMALIZE divided by the sum of the chosen s first (0 where that is
  * 0).  The order is that of the exact ranks: fp32 scores too close to tell apart are
  * ranked again in 64 bits, and without a bias the logits themselves are compared.
- * A logit of -inf masks its expert: it is never chosen, and choices for which no
- * expert is left get id -1 and weight 0.  A NaN ranks first; in a softmax row a NaN or
+ * A logit of -inf masks its expert, and so does a bias of -inf (which leaves it in a
+ * softmax row's total): it is never chosen, and choices for which no expert is left get
+ * id -1 and weight 0.  A bias of +inf ranks its expert before all finite ones.  A NaN ranks first; in a softmax row a NaN or
  * +inf makes every score NaN.  Both outputs contiguous. */
 #define TTN_ROUTE_SIGMOID 1u
 #define TTN_ROUTE_RENORMALIZE 2u

@@ -52,6 +52,8 @@ def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, 
             s = {e: math.nan if math.isnan(v[e]) else 1 / (1 + math.exp(-v[e])) if v[e] > -700 else math.exp(v[e])
                  for e in open_}
         rank = {e: s[e] + (0.0 if bias is None else float(bias[e])) for e in open_}
+        open_ = [e for e in open_ if rank[e] != -math.inf]  # a bias of -inf masks an expert as a logit does
+        rank = {e: rank[e] for e in open_}
         if groups > 1:
             size = experts // groups
             strength = []

@@ -99,7 +99,7 @@ __device__ double exact_rank(const RouteArgs& a, int64_t row, int e, float m, do
   if (x == -HUGE_VAL) return x;
   if (a.by_logit) return m != m ? (double)m : x;  // m is NaN in a softmax row with a NaN or +inf
   double s = a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - (double)m) / total;
-  return a.bias ? s + (double)a.bias[e] : s;
+  return a.bias ? s + (double)a.bias[e] : s;  // -inf with a bias of -inf: never chosen
 }
 
 // The choice of one row in 64 bits throughout: lane j gets the expert of choice j (or -1).
@@ -269,7 +269,8 @@ __global__ void __launch_bounds__(kRouteThreads, W <= 8 ? 12 : 4) route_rows(Rou
       const uint32_t out = __ballot_sync(kAll, lane < a.groups && rank == a.top_groups);
       const float inner = __shfl_sync(kAll, strength, __ffs(in) - 1);
       const float outer = __shfl_sync(kAll, strength, __ffs(out) - 1);
-      if (inner - outer <= band * fmaxf(1.0f, fabsf(inner))) {  // not so for infinities
+      // an infinite rank (a bias of +-inf) is the same in any precision
+      if (fabsf(inner) < __int_as_float(0x7f800000) && inner - outer <= band * fmaxf(1.0f, fabsf(inner))) {
         // The last group kept and the first left out are too close for fp32: the experts that can
         // be among their group's group_top, one a lane, ranked in 64 bits.
         const float least = a.group_top == 2 && t2 != ninf ? t2 : t1;
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(kRouteThreads, W <= 8 ? 12 : 4) route_rows(Rou
 #pragma unroll
         for (int i = 0; i < W; ++i) {
           const float bar = __shfl_sync(kAll, least, min(first + i, a.experts - 1) / a.group_size);
-          const bool can = v[i] != ninf && v[i] >= bar - band * fmaxf(1.0f, fabsf(bar));
+          const bool can = v[i] != ninf && (v[i] >= bar || v[i] >= bar - band * fmaxf(1.0f, fabsf(bar)));  // bar: +inf too
           const uint32_t vote = __ballot_sync(kAll, can);
           const int at = n + __popc(vote & ((1u << lane) - 1));
           if (can && at < 32) packed[warp][at].y = __int_as_float(first + i);

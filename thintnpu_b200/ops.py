@@ -683,8 +683,8 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     best rank (``group_top`` 1) or sum of two best ranks (2) is largest.  The ``top_k``
     (at most 16) best come in falling rank, ties to the lower index, ranked as their
     exact values are; their weights are the scores (without the bias), divided by their
-    sum with ``renormalize``, times ``scale``.  Logits of -inf are never chosen: places
-    for which no expert is left hold id -1 and weight 0.  ``out`` is a (weights, experts)
+    sum with ``renormalize``, times ``scale``.  Experts with a logit or a bias of
+    -inf are never chosen: places for which no expert is left hold id -1 and weight 0.  ``out`` is a (weights, experts)
     pair to fill."""
     what = "route_experts"
     dtype = _check_rows(logits, what)
