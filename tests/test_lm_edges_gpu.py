@@ -13,6 +13,31 @@ pytestmark = pytest.mark.gpu
 
 # ------------------------------------------------------------------ route_experts
 
+@pytest.mark.parametrize("size", [3, 4])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("large", [64.0, 1000.0, 1e5])
+def test_route_group_sums_of_large_biases_that_cancel(device, size, score, large):
+    """A group's two best ranks are near +large and -large: their FP32 sum's error goes with
+    the ranks, not with the sum, and group sums differ by less than that."""
+    g = torch.Generator().manual_seed(int(large) + size)
+    rows, groups = 256, 8
+    if score == "sigmoid":
+        first = 0.3 + 0.4 * torch.rand(rows, groups, 1, generator=g, dtype=torch.float64)
+        second = 1.0 - first + torch.randint(-40, 41, (rows, groups, 1), generator=g) * 2.0 ** -21
+        rest = 0.5 * torch.ones(rows, groups, size - 2, dtype=torch.float64)
+        s = torch.cat((first, second, rest), 2)
+        logits = torch.log(s / (1 - s)).float().view(rows, groups * size)
+    else:
+        pair = 1.0 / (2 * groups) + torch.randint(-40, 41, (rows, groups, 2), generator=g) * 2.0 ** -22
+        rest = 1e-6 * torch.ones(rows, groups, size - 2, dtype=torch.float64)
+        logits = torch.log(torch.cat((pair, rest), 2)).float().view(rows, groups * size)
+    bias = torch.cat((torch.full((groups, 1), large), torch.full((groups, 1), -large),
+                      torch.full((groups, size - 2), -4 * large)), 1).reshape(-1)
+    for top_groups in (1, 4):
+        check_route(device, logits, 4, score=score, bias=bias, groups=groups, top_groups=top_groups, group_top=2,
+                    renormalize=True)
+
+
 @pytest.mark.parametrize("experts,groups", [(32, 8), (24, 8), (256, 8), (60, 4)])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_route_infinite_biases(device, experts, groups, score):

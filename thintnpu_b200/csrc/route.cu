@@ -13,7 +13,7 @@
 // rise with x, so without a bias the rank is x itself.  With a bias (or a group's sum of
 // two scores) ranks are fp32 sums with an error below rank_band; neighbours in the chosen
 // order that lie closer than that are ranked again in 64 bits, one candidate a lane, and so
-// are the groups' best where the last group kept and the first left out are that close.  On
+// are the groups' best where a group kept and one left out are that close.  On
 // N(0, 1.5) logits with 256 experts about one row in two hundred has such neighbours.
 //
 // Bound: a row of 256 fp32 logits is 1 KB of reading (0.16 us a thousand rows at copy
@@ -35,8 +35,11 @@ constexpr uint32_t kAll = 0xffffffffu;
 // values.  With u = 2^-24: a sigmoid score is within 8 u (exp2 and reciprocal approximations
 // of 2 ulp, the argument's rounding, 1 + e); a softmax score within (W + 19) u, as its
 // total of W terms a lane and five shuffles rounds W + 4 times and each term is within 6 u
-// (s |x - m| <= 0.37).  The bias addition rounds by |rank| u more; a difference doubles that
-// and a group's sum of two doubles it again.
+// (s |x - m| <= 0.37).  The bias addition rounds by |rank| u more; a difference of two doubles
+// that.  A group's strength, the sum of two ranks r and q, is within twice a score's error and
+// (|r| + |q| + |r + q|) u, which large biases of opposite sign leave far above |r + q| u, and its
+// sum with that bound rounds once more: 0.6 band * max(1, |r| + |q|) bounds it (with band = 36 u:
+// 16 + 3 (|r| + |q|) <= 19 max(1, |r| + |q|)).
 template <int W>
 __device__ __forceinline__ float rank_band(bool sigmoid) {
   return (sigmoid ? 4.0f * 9.0f : 4.0f * (W + 20.0f)) * 5.9604645e-8f;
@@ -265,13 +268,13 @@ __global__ void __launch_bounds__(kRouteThreads, W <= 8 ? 12 : 4) route_rows(Rou
     }
     uint32_t kept = __ballot_sync(kAll, lane < a.groups && rank < a.top_groups);
     if (!a.by_logit) {
-      const uint32_t in = __ballot_sync(kAll, lane < a.groups && rank == a.top_groups - 1);
-      const uint32_t out = __ballot_sync(kAll, lane < a.groups && rank == a.top_groups);
-      const float inner = __shfl_sync(kAll, strength, __ffs(in) - 1);
-      const float outer = __shfl_sync(kAll, strength, __ffs(out) - 1);
-      // an infinite rank (a bias of +-inf) is the same in any precision
-      if (fabsf(inner) < __int_as_float(0x7f800000) && inner - outer <= band * fmaxf(1.0f, fabsf(inner))) {
-        // The last group kept and the first left out are too close for fp32: the experts that can
+      // how far the strength may be off; an infinite rank is the same in any precision
+      const float size = a.group_top == 2 && t2 != ninf ? fabsf(t1) + fabsf(t2) : fabsf(t1);
+      const float off = fabsf(strength) < __int_as_float(0x7f800000) ? 0.6f * band * fmaxf(1.0f, size) : 0.0f;
+      const float least_kept = -warp_largest(kept >> lane & 1u ? off - strength : ninf);
+      const float most_left = warp_largest(kept >> lane & 1u ? ninf : strength + off);
+      if (most_left != ninf && least_kept <= most_left) {
+        // A group kept and one left out are too close for fp32: the experts that can
         // be among their group's group_top, one a lane, ranked in 64 bits.
         const float least = a.group_top == 2 && t2 != ninf ? t2 : t1;
         int n = 0;
