@@ -57,3 +57,19 @@ def test_route_infinite_biases(device, experts, groups, score):
             for top_groups in (1, 3):
                 check_route(device, logits, 3, score=score, bias=bias, groups=groups, top_groups=top_groups,
                             group_top=group_top, renormalize=True)
+
+
+@pytest.mark.parametrize("experts", [12, 16])
+def test_route_group_sums_beyond_the_largest_float(device, experts):
+    """Two ranks of the lowest finite value sum to less than FP32 holds; a group of them is still
+    ahead of a group in which everything is masked."""
+    groups, size, low = 4, experts // 4, torch.finfo(torch.float32).min
+    logits = torch.randn(5, experts, generator=torch.Generator().manual_seed(3))
+    logits[:, :size] = -math.inf
+    bias = torch.zeros(experts)
+    bias[2 * size:] = low
+    check_route(device, logits, size + 2, score="sigmoid", bias=bias, groups=groups, top_groups=2, group_top=2)
+    bias[2 * size:] = 0.0
+    bias[size:2 * size] = -low
+    bias[3 * size:] = -low
+    check_route(device, logits, 3, score="sigmoid", bias=bias, groups=groups, top_groups=1, group_top=2)

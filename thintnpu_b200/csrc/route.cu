@@ -260,7 +260,10 @@ __global__ void __launch_bounds__(kRouteThreads, W <= 8 ? 12 : 4) route_rows(Rou
           t1 = fmaxf(t1, k[e]);
         }
     }
-    const float strength = lane >= a.groups ? ninf : a.group_top == 2 && t2 != ninf ? t1 + t2 : t1;
+    // two ranks are added as halves: the sum of two finite ones stays finite
+    const bool two = a.group_top == 2 && t2 != ninf;
+    const float half = a.group_top == 2 ? 0.5f : 1.0f;
+    const float strength = lane >= a.groups ? ninf : two ? 0.5f * t1 + 0.5f * t2 : half * t1;
     int rank = 0;
     for (int g = 0; g < a.groups; ++g) {
       const float o = __shfl_sync(kAll, strength, g);
@@ -269,14 +272,14 @@ __global__ void __launch_bounds__(kRouteThreads, W <= 8 ? 12 : 4) route_rows(Rou
     uint32_t kept = __ballot_sync(kAll, lane < a.groups && rank < a.top_groups);
     if (!a.by_logit) {
       // how far the strength may be off; an infinite rank is the same in any precision
-      const float size = a.group_top == 2 && t2 != ninf ? fabsf(t1) + fabsf(t2) : fabsf(t1);
-      const float off = fabsf(strength) < __int_as_float(0x7f800000) ? 0.6f * band * fmaxf(1.0f, size) : 0.0f;
+      const float size = two ? 0.5f * fabsf(t1) + 0.5f * fabsf(t2) : half * fabsf(t1);
+      const float off = fabsf(strength) < __int_as_float(0x7f800000) ? 0.6f * band * fmaxf(half, size) : 0.0f;
       const float least_kept = -warp_largest(kept >> lane & 1u ? off - strength : ninf);
       const float most_left = warp_largest(kept >> lane & 1u ? ninf : strength + off);
       if (most_left != ninf && least_kept <= most_left) {
         // A group kept and one left out are too close for fp32: the experts that can
         // be among their group's group_top, one a lane, ranked in 64 bits.
-        const float least = a.group_top == 2 && t2 != ninf ? t2 : t1;
+        const float least = two ? t2 : t1;
         int n = 0;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
@@ -528,10 +531,10 @@ extern "C" ttn_status ttn_route_experts(const ttn_tensor* logits, const float* b
   a.groups = top_groups == groups ? 1 : (int)groups;  // all groups kept: none matter
   a.group_size = (int)(e / a.groups);
   a.top_groups = (int)top_groups;
-  a.group_top = group_top;
+  a.group_top = a.group_size == 1 ? 1 : group_top;
   a.sigmoid = flags & TTN_ROUTE_SIGMOID ? 1 : 0;
   a.renormalize = flags & TTN_ROUTE_RENORMALIZE ? 1 : 0;
-  a.by_logit = !bias && (a.groups == 1 || group_top == 1 || a.group_size == 1);
+  a.by_logit = !bias && (a.groups == 1 || a.group_top == 1);
   const int64_t size = row_dtype_size(logits->dtype);
   a.vec = a.col_stride == 1 && a.width * size % 16 == 0 && (uintptr_t)logits->data % 16 == 0 &&
           a.row_stride * size % 16 == 0;
