@@ -448,8 +448,7 @@ ttn_status ttn_token_logprobs(const ttn_tensor* logits, const int64_t* tokens, f
  * (-1: no choice; another rank's experts) add nothing; a token without any other id
  * gets zeros.  Products accumulate in FP32; the gated activations are rounded to dtype
  * between the two products where the tensor cores take them (so they have to lie in its
- * range), and each pair's share of an output to 2^-15 of the largest of its 32 neighbours;
- * with few pairs neither.  hidden % 8 == 0, inner % 16 == 0 (both up to 2^20),
+ * range), with few pairs not.  hidden % 8 == 0, inner % 16 == 0 (both up to 2^20),
  * num_experts 1..1024, top_k 1..32, tokens * top_k <= (2^31 - 1) / 256; 16-byte aligned
  * bases, row strides multiples of 8 and at least hidden.  workspace: at least
  * ttn_expert_mlp_workspace_size bytes (0 for malformed sizes), 256-byte aligned, used by

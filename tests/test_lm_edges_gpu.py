@@ -7,9 +7,46 @@ import math
 import pytest
 import torch
 
-from test_lm_gpu import check_route
+from oracle import lm
+from test_lm_gpu import check_mlp, check_route, mlp_inputs
 
 pytestmark = pytest.mark.gpu
+
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+# ------------------------------------------------------------------ expert_mlp
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", [(60, 96, 64, 4, 2), (300, 96, 64, 3, 1),
+                                                                (420, 200, 48, 6, 3), (2400, 72, 2048, 2, 2)])
+def test_mlp_features_far_apart_keep_their_own_precision(device, dtype, tokens, hidden, inner, experts, top_k):
+    """One output feature in 32 is 10^4 times its neighbours, as massive features of a
+    down projection are: the neighbours' error is bounded by their own sums alone."""
+    import thintnpu_b200 as ttn
+    args = mlp_inputs(tokens, hidden, inner, experts, top_k, DTYPES[dtype], 77)
+    args[4][:, 5::32] = (args[4][:, 5::32].double() * 1e4).to(DTYPES[dtype])
+    check_mlp(ttn.expert_mlp(*(t.to(device) for t in args)), args)
+
+
+@pytest.mark.parametrize("tokens", [40, 300])
+@pytest.mark.parametrize("peak", [2.0 ** 125, 2.0 ** 126.5, 3.2e38])
+def test_mlp_shares_near_the_largest_float(device, tokens, peak):
+    """Shares up to FP32's largest values with routing weights that bring them back.  All
+    factors are positive, so no partial sum is larger than its share."""
+    import thintnpu_b200 as ttn
+    x, ids, weights, gate_up, down = (t.abs() if t.is_floating_point() else t
+                                      for t in mlp_inputs(tokens, 64, 32, 3, 2, torch.bfloat16, 19))
+    one = torch.ones(tokens, 1)
+    largest = max(float(lm.expert_mlp(x, torch.full((tokens, 1), e, dtype=torch.int32), one, gate_up, down)[0].max())
+                  for e in range(3))
+    # bf16 rounds a factor by 2^-9, the shares' FP32 sums by far less
+    down = (down.double() * (peak * (1 - 2.0 ** -6) / largest)).bfloat16()
+    args = (x, ids, weights * 2.0 ** -12, gate_up, down)
+    got = ttn.expert_mlp(*(t.to(device) for t in args))
+    assert bool((got > 0).all())
+    check_mlp(got, args)
+
 
 # ------------------------------------------------------------------ route_experts
 

@@ -18,9 +18,10 @@
 //      one TMA box of a five-dimensional map, so that the gate and up values of a feature
 //      sit in lanes l and l + 16 of one warp: one shuffle a value pair, then
 //      silu(gate) * up, rounded to the operands' type for the second product.
-//    - The second product's values, one pair's share of an output, are kept in 16 bits:
-//      integers times an FP32 scale for each 32 features of a pair (a warp's lanes), exact
-//      to 2^-16 of the largest of the 32, where a rounding to bf16 would be off by 2^-9.
+//    - The second product's values, one pair's share of an output, stay FP32: they are terms of
+//      a sum, and neighbouring features may be orders of magnitude apart.  8192 tokens x 8, hidden
+//      2048: second product 268 us and combine 92 us, where 16-bit integers under one scale for 32
+//      features (0.5 GB less traffic) took 258 and 66.
 //  * expert_combine adds a token's shares in the order of its choices.
 // Every wait is bounded (200 ms); a role that gives up records why in a device word
 // (ttn_expert_mlp_fault) and the pair frees its TMEM and returns.
@@ -258,22 +259,18 @@ constexpr int epi_warps(bool gate_up) { return gate_up ? 12 : 8; }
 constexpr int kGatherWarps = 4;  // of the first product
 constexpr int kGatherRows = kTileN / 2 / kGatherWarps;
 constexpr int product_threads(bool gate_up) { return 64 + 32 * epi_warps(gate_up) + (gate_up ? 32 * kGatherWarps : 0); }
-constexpr int kStagingPitch = 36;  // words: conflict-free both ways
-// one epilogue warp: 32 rows x 16 activations, or 16 rows x 32 values
-constexpr uint32_t staging_bytes(bool gate_up) { return gate_up ? 32 * 16 * 2 : 16 * kStagingPitch * 4; }
-constexpr int kShareBlock = 32;              // features that share a scale
+// one epilogue warp of the first product: 32 rows x 16 activations
+constexpr uint32_t staging_bytes(bool gate_up) { return gate_up ? 32 * 16 * 2 : 0; }
 
 struct ProductArgs {
   int32_t *offsets, *order;
   const int32_t* ids;  // gate-up: sort these pairs here (block 0 leaves the result); null: they are sorted
   int pairs;
   uint16_t* h;      // gate-up: [pairs, sorted][inner]
-  int16_t* share;   // down: [pair][hidden], integers (or bf16 where the scale is negative)
-  float* scale;     // down: [pair][blocks]
-  int experts, top_k, rows, steps, m_tiles, blocks;  // rows: weight rows of the product (inner or hidden)
+  float* share;     // down: [pair][hidden]
+  int experts, top_k, rows, steps, m_tiles;  // rows: weight rows of the product (inner or hidden)
   int bf16;
   int withhold;     // test hook: no operand copy, so every other role's first wait runs out
-  int wide;         // down: share rows are multiples of 32 bytes
 };
 // Up to this many pairs every block of the first product sorts them for itself instead of a
 // launch of expert_plan (3 us of the host's time a call).  With the launch / without, us: 512
@@ -633,56 +630,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
             __syncwarp();
           }
         } else {
-          // 16 columns at a time through shared memory: two lanes a row then hold 16 neighbouring
-          // features each, so the row's largest is found in registers (a warp-wide reduction a
-          // column made this epilogue 200 cycles a column and the product 434 us, now 258 us).
-          const int f0 = tile * 256 + (int)rank * 128 + quarter * 32;
-          const int n = lane >> 1, f = f0 + (lane & 1) * 16;
-          uint32_t* in = reinterpret_cast<uint32_t*>(own) + lane;
-          const uint4* back = reinterpret_cast<const uint4*>(own) + (n * kStagingPitch + (lane & 1) * 16) / 4;
-          for (int c = group * 16; c < rows && f0 < a.rows; c += kEpiGroups * 16) {
-            const int pair = c + n < rows ? order[row0 + c + n] : -1;
-            uint32_t r[16];
-            tmem_ld16(lanes + acc * kTileN + c, r);
+          // A lane has one feature of 32 pairs: each pair's 32 features are one 128-byte line.
+          const int f = tile * 256 + (int)rank * 128 + quarter * 32 + lane;
+          for (int c = group * 32; c < rows && f - lane < a.rows; c += kEpiGroups * 32) {
+            const int own_pair = c + lane < rows ? order[row0 + c + lane] : 0;
+            uint32_t r[32];
+            tmem_ld32(lanes + acc * kTileN + c, r);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) in[i * kStagingPitch] = r[i];
-            __syncwarp();
-            uint32_t v[16], top = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint4 q = back[i];
-              v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
+            for (int i = 0; i < 32; ++i) {
+              const int pair = __shfl_sync(kAll, own_pair, i);
+              if (c + i < rows && f < a.rows) a.share[(int64_t)pair * a.rows + f] = __uint_as_float(r[i]);
             }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = max(top, v[i] & 0x7fffffffu);
-            top = max(top, __shfl_xor_sync(kAll, top, 1));
-            const float peak = __uint_as_float(top);
-            const bool whole = peak >= 1e-30f && top < 0x7f800000u;
-            const float inverse = __fdividef(32767.0f, peak);
-            uint32_t w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float lo = __uint_as_float(v[2 * i]), hi = __uint_as_float(v[2 * i + 1]);
-              // adding 1.5 * 2^23 rounds to an integer and leaves it in the low bits
-              w[i] = __byte_perm(__float_as_uint(fmaf(lo, inverse, 12582912.0f)),
-                                 __float_as_uint(fmaf(hi, inverse, 12582912.0f)), 0x5410);
-            }
-            if (!whole) {  // zeros, vanishing values, infinities, NaN: as bf16
-#pragma unroll
-              for (int i = 0; i < 8; ++i) w[i] = BF16::round2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-            }
-            if (pair >= 0) {
-              if ((lane & 1) == 0) a.scale[(int64_t)pair * a.blocks + f0 / kShareBlock] = whole ? peak * (1.0f / 32767.0f) : -1.0f;
-              int16_t* to = a.share + (int64_t)pair * a.rows + f;
-              if (a.wide) {  // rows of whole 32-byte sectors
-                if (f < a.rows) store32(to, w);
-              } else {
-                if (f < a.rows) reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                if (f + 8 < a.rows) reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-              }
-            }
-            __syncwarp();
           }
         }
         tc_fence_before();
@@ -704,27 +662,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
   if (warp == 1) tmem_pair_dealloc(tmem, 2 * kTileN);
 }
 
-// out[token] = sum of weight * share over the token's choices, in their order; 8 features a thread.
+// out[token] = sum of weight * share over the token's choices, in their order; 4 features a thread.
 constexpr int kCombineThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(kCombineThreads, 4) expert_combine(ExpertArgs a, const int16_t* __restrict__ share,
-                                                                  const float* __restrict__ scale, int blocks,
+__global__ void __launch_bounds__(kCombineThreads, 3) expert_combine(ExpertArgs a, const float* __restrict__ share,
                                                                   FastDiv groups) {
   pdl_trigger();
   pdl_wait();
   const uint32_t i = blockIdx.x * kCombineThreads + threadIdx.x;
-  const uint32_t token = groups.div(i), f = (i - token * groups.d) * 8;
+  const uint32_t token = groups.div(i), f = (i - token * groups.d) * 4;
   if (token >= a.tokens) return;
-  unsigned long long sum[4] = {};  // pairs of features (packed arithmetic)
-  constexpr int kBatch = 8;        // choices whose loads are in flight together
+  float sum[4] = {};
+  constexpr int kBatch = 8;  // choices whose loads are in flight together
   for (int j0 = 0; j0 < a.top_k; j0 += kBatch) {
     const int64_t pair0 = (int64_t)token * a.top_k + j0;
     const int32_t* ids = a.ids + pair0;
     const float* weights = a.weights + pair0;
-    const int16_t* from = share + pair0 * a.hidden + f;
-    const float* scales = scale + pair0 * blocks + f / kShareBlock;
-    float w[kBatch], sc[kBatch];
-    uint4 v[kBatch];
+    const float* from = share + pair0 * a.hidden + f;
+    float w[kBatch];
+    float4 v[kBatch];
     uint32_t live = 0;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)  // shares of pairs without an expert were never written
@@ -732,40 +688,19 @@ __global__ void __launch_bounds__(kCombineThreads, 4) expert_combine(ExpertArgs 
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       if (!(live >> j & 1u)) continue;
-      v[j] = __ldcs(reinterpret_cast<const uint4*>(from + (int64_t)j * a.hidden));
+      v[j] = __ldcs(reinterpret_cast<const float4*>(from + (int64_t)j * a.hidden));
       w[j] = weights[j];
-      sc[j] = scales[(int64_t)j * blocks];
     }
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       if (!(live >> j & 1u)) continue;
-      const uint32_t words[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-      const bool whole = sc[j] >= 0.0f;
-      const float by = whole ? w[j] * sc[j] : w[j];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        unsigned long long p;
-        if (whole) {
-          // i -> the FP32 of bits 0x4b000000 + (i + 2^15), which is 2^23 + 2^15 + i
-          const uint32_t u = words[q] ^ 0x80008000u;
-          p = f2_add(f2_pack(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7610)),
-                             __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7632))),
-                     f2_pack(-8421376.0f, -8421376.0f));
-        } else {
-          const float2 b = BF16::two(words[q]);
-          p = f2_pack(b.x, b.y);
-        }
-        sum[q] = f2_fma(p, f2_pack(by, by), sum[q]);
-      }
+      sum[0] = fmaf(w[j], v[j].x, sum[0]);
+      sum[1] = fmaf(w[j], v[j].y, sum[1]);
+      sum[2] = fmaf(w[j], v[j].z, sum[2]);
+      sum[3] = fmaf(w[j], v[j].w, sum[3]);
     }
   }
-  uint32_t out[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const float2 p = f2_unpack(sum[q]);
-    out[q] = T::round2(p.x, p.y);
-  }
-  *reinterpret_cast<uint4*>(a.out + token * a.out_stride + f) = make_uint4(out[0], out[1], out[2], out[3]);
+  *reinterpret_cast<uint2*>(a.out + token * a.out_stride + f) = make_uint2(T::round2(sum[0], sum[1]), T::round2(sum[2], sum[3]));
 }
 
 // Whether each pair reads its expert's weights by itself, on ordinary warps: where all those
@@ -793,9 +728,9 @@ bool two_subs(int64_t pairs, int64_t experts, int64_t inner) {
 }
 
 struct Sizes {
-  int64_t pairs, blocks;
-  bool rows;                                 // the few-pairs kernels
-  int64_t order, h, share, scale, total;     // byte offsets into the workspace (offsets at 0)
+  int64_t pairs;
+  bool rows;                        // the few-pairs kernels
+  int64_t order, h, share, total;   // byte offsets into the workspace (offsets at 0)
 };
 bool sizes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64_t top_k, Sizes* s) {
   if (tokens < 0 || hidden < 1 || inner < 1 || experts < 1 || experts > kMaxExperts || top_k < 1 ||
@@ -803,17 +738,15 @@ bool sizes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64
     return false;
   auto pad = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
   s->pairs = tokens * top_k;
-  s->blocks = (hidden + kShareBlock - 1) / kShareBlock;
   s->rows = few_pairs(s->pairs, hidden, inner, experts);
   if (s->rows) {
-    s->order = s->h = s->share = s->scale = 0;
+    s->order = s->h = s->share = 0;
     s->total = pad(s->pairs * inner * 4);
   } else {
     s->order = pad((experts + 1) * 4);
     s->h = s->order + pad(s->pairs * 4);
     s->share = s->h + pad(s->pairs * inner * 2);
-    s->scale = s->share + pad(s->pairs * hidden * 2);
-    s->total = s->scale + pad(s->pairs * s->blocks * 4);
+    s->total = s->share + pad(s->pairs * hidden * 4);
   }
   return true;
 }
@@ -836,8 +769,7 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
   constexpr bool bf16 = std::is_same<T, BF16>::value;
   int32_t *offsets = (int32_t*)ws, *order = (int32_t*)(ws + s.order);
   uint16_t* h = (uint16_t*)(ws + s.h);
-  int16_t* share = (int16_t*)(ws + s.share);
-  float* scale = (float*)(ws + s.scale);
+  float* share = (float*)(ws + s.share);
   const cuuint64_t hidden = a.hidden, inner = a.inner, experts = a.experts;
   ProductMaps gate, down;
   {  // gate-up weights: (hidden, 16 rows, gate | up, inner / 16, expert)
@@ -874,15 +806,13 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     const int tile = (gate_up ? 128 : 256) * subs;  // features of a tile
     const uint32_t smem = product_smem(gate_up, a.experts);
     ProductArgs p = {};
-    p.offsets = offsets, p.order = order, p.h = h, p.share = share, p.scale = scale;
+    p.offsets = offsets, p.order = order, p.h = h, p.share = share;
     p.ids = here && gate_up ? a.ids : nullptr, p.pairs = (int)s.pairs;
     p.experts = a.experts, p.top_k = a.top_k, p.rows = rows;
     p.steps = (length + kStepK - 1) / kStepK;
     p.m_tiles = (rows + tile - 1) / tile;
-    p.blocks = (int)s.blocks;
     p.bf16 = bf16;
     p.withhold = gate_up && g_withhold_next_products.exchange(false);
-    p.wide = a.hidden % 16 == 0;
     if (runs * p.m_tiles > INT32_MAX) return fail(TTN_UNSUPPORTED, "%s: more than 2^31 tiles", name);
     TTN_TRY(ensure_dynamic_smem((const void*)kernel, (int)smem));
     const int64_t pairs_of_sms = sm_count() / 2, most = runs * p.m_tiles;
@@ -894,11 +824,11 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
   else
     TTN_TRY(products(expert_products<T, true, 1>, true, 1, gate, a.inner, a.hidden));
   TTN_TRY(products(expert_products<T, false, 1>, false, 1, down, a.hidden, a.inner));
-  const int64_t items = a.tokens * (a.hidden / 8);
+  const int64_t items = a.tokens * (a.hidden / 4);
   if (items + kCombineThreads > UINT32_MAX) return fail(TTN_UNSUPPORTED, "%s: output too large", name);
   return cuda_check(launch_pdl(expert_combine<T>, dim3((unsigned)((items + kCombineThreads - 1) / kCombineThreads)),
-                               dim3(kCombineThreads), 0, stream, a, (const int16_t*)share, (const float*)scale,
-                               (int)s.blocks, FastDiv((uint32_t)(a.hidden / 8))),
+                               dim3(kCombineThreads), 0, stream, a, (const float*)share,
+                               FastDiv((uint32_t)(a.hidden / 4))),
                     name);
 }
 

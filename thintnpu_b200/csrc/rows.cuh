@@ -99,13 +99,6 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-// One 32-byte store; the address must be 32-byte aligned.
-__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-               : "memory");
-}
-
 inline bool row_dtype(int dtype) { return dtype == TTN_F16 || dtype == TTN_F32 || dtype == TTN_BF16; }
 inline int64_t row_dtype_size(int dtype) { return dtype == TTN_F32 ? 4 : 2; }
 
