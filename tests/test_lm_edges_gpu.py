@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import lm
-from test_lm_gpu import check_mlp, check_route, mlp_inputs
+from test_lm_gpu import check_logprobs, check_mlp, check_route, mlp_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,38 @@ def test_route_group_sums_beyond_the_largest_float(device, experts):
     bias[size:2 * size] = -low
     bias[3 * size:] = -low
     check_route(device, logits, 3, score="sigmoid", bias=bias, groups=groups, top_groups=1, group_top=2)
+
+
+# ------------------------------------------------------------------ token_logprobs
+
+@pytest.mark.parametrize("vocabulary,top", [(40, 8), (5000, 20)])
+@pytest.mark.parametrize("size", [2.0 ** 18, 2.0 ** 21, 1e7, 3e8, 1e9, 1e10, 1e15, 1e20, 1e30, 3e38])
+def test_logprobs_far_from_zero(device, size, vocabulary, top):
+    """Rows whose largest logit is far from zero on either side, where the scaled maximum has
+    no bits left for what separates its neighbours."""
+    g = torch.Generator().manual_seed(vocabulary)
+    step = size * 2.0 ** -23  # of an FP32 logit
+    near = torch.randint(0, 8, (6, vocabulary), generator=g).double() * max(step, 0.5)
+    rows = torch.randn(6, vocabulary, generator=g).double()
+    rows[0] = -size                                     # everything under a finite mask
+    rows[1] = size
+    rows[2] = -size - near[2] if size < 1e38 else -size
+    rows[3] = size - near[3]
+    rows[4, ::7] = size                                 # beside ordinary ones
+    rows[5] = -size
+    rows[5, 1::9] = -size / 2
+    for dtype, scale in (("f32", 1.0), ("f32", 0.3), ("bf16", 1.0)):
+        logits = rows.clamp(-3.38e38, 3.38e38).to(DTYPES[dtype])
+        check_logprobs(device, logits, torch.randint(vocabulary, (6,), generator=g), top, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [1e-6, 1e3, 1e6])
+def test_logprobs_extreme_scales(device, dtype, scale):
+    g = torch.Generator().manual_seed(4)
+    rows = torch.randn(6, 3000, generator=g) / min(scale, 1e3)
+    rows[1:3] = 60000.0 * torch.randn(2, 3000, generator=g).clamp(-1, 1)
+    rows[3] = -54321.0
+    rows[4] = 33333.0
+    logits = rows.to(DTYPES[dtype])
+    check_logprobs(device, logits, torch.randint(3000, (6,), generator=g), 20, scale=scale)

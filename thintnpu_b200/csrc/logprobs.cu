@@ -1,24 +1,21 @@
 // Log probabilities of given tokens, entropy and the largest alternatives of vocabulary
 // rows, in one pass over the logits.
 //
-// With c = scale log2 e and M = c times the running maximum, rounded once, t = c x - M (one
-// fused multiply-add, so its error is |t| 2^-24 however large x is): S = sum 2^t and
-// A = sum 2^t t are kept in FP32 and rescaled by differences of M when the maximum rises.
-// log2 p(x) = t - log2 S, and the entropy is log2 S - A / S in units of log 2 (both terms
-// >= 0 but for the rounding of M: no cancellation).
+// With c = scale log2 e and t = c (x - the running maximum): S = sum 2^t and A = sum 2^t t are
+// kept in FP32 and rescaled when the maximum rises.  log2 p(x) = t - log2 S, and the entropy is
+// log2 S - A / S in units of log 2 (both terms >= 0: no cancellation).  The difference comes
+// first, so that t's error is 2^-23 |t| at most however large x is (finite masks such as -1e10,
+// the lowest values); one fused multiply-add with a rounded c * maximum saves half an instruction
+// a logit (4096 x 128,000 bf16: 208 us for 212) but is off by 2^-24 c |x|.
 //
 // The alternatives ride along.  A warp reads segments of 64 16-byte vectors (512 16-bit
-// logits) and needs their maxima for M anyway; it leaves them in shared memory.  The n-th
+// logits) and needs their maxima anyway; it leaves them in shared memory.  The n-th
 // largest of 32 lanes' maxima over those is a floor: n elements are at least that large, so
 // the n largest of the row lie in the segments whose maximum reaches it.  Only those (about
 // 30 of 250 for n = 20) are read again (they are in L2), and their elements from the floor
 // up, usually n to 2n, are put in order by counting the larger ones.
 //
-// Where the maximum's magnitude is 2^100 or more, c x would overflow; c is 2^-60 there.
-// Values that differ at all then differ by 2^77 or more, so all but those equal to the
-// maximum vanish with it as they do with any allowed scale (>= 1e-6), and M is exact.
-//
-// A row is read by a cluster of 1 to 8 CTAs, one slice each; CTA 0 joins their (m, S, A)
+// A row is read by a cluster of 1 to 8 CTAs, one slice each; CTA 0 joins their (maximum, S, A)
 // and their sorted lists through distributed shared memory.
 //
 // Bound: the row's bytes; the arithmetic (about 8 instructions and one exp2 a logit) has
@@ -90,25 +87,22 @@ __device__ __noinline__ K merge32(K list, K other, int lane) {
   return v;
 }
 struct LpPart {  // what a warp or a CTA knows of its part of the row
-  float m, s, a;     // M, S, A
+  float s, a;        // S, A
   uint32_t top_key;  // key of the largest logit
 };
-// The factor of logits whose maximum is `most`.
-__device__ __forceinline__ float factor(float most, float c) {
-  return fabsf(most) < 1.2676506e30f ? c : 8.6736174e-19f;  // 2^100, 2^-60
-}
+// What takes a t of the maximum `from` to one of the maximum `to`, no further than where 2^t is 0.
+__device__ __forceinline__ float apart(float from, float to, float c) { return fmaxf((from - to) * c, -256.0f); }
 // b joined to a: both rescaled to the larger maximum.  A part without live logits has s = 0.
 __device__ __forceinline__ LpPart join(const LpPart& a, const LpPart& b, float c) {
   LpPart r;
   r.top_key = max(a.top_key, b.top_key);
-  if (b.s == 0.0f || a.s == 0.0f || factor(key_value(a.top_key), c) != factor(key_value(b.top_key), c)) {
-    // one has nothing, or nothing beside the other
-    const LpPart& o = b.s == 0.0f || (a.s != 0.0f && a.top_key > b.top_key) ? a : b;
-    r.m = o.m, r.s = o.s, r.a = o.a;
+  if (b.s == 0.0f || a.s == 0.0f) {  // one has nothing
+    const LpPart& o = b.s == 0.0f ? a : b;
+    r.s = o.s, r.a = o.a;
     return r;
   }
-  r.m = fmaxf(a.m, b.m);
-  const float ta = fmaxf(a.m - r.m, -256.0f), tb = fmaxf(b.m - r.m, -256.0f);
+  const float most = key_value(r.top_key);
+  const float ta = apart(key_value(a.top_key), most, c), tb = apart(key_value(b.top_key), most, c);
   const float fa = exp2f(ta), fb = exp2f(tb);
   r.s = a.s * fa + b.s * fb;
   r.a = (a.a + a.s * ta) * fa + (b.a + b.s * tb) * fb;
@@ -118,7 +112,7 @@ __device__ __forceinline__ LpPart join(const LpPart& a, const LpPart& b, float c
 // Joins the parts of the first `count` lanes (a power of two), pairwise; lane 0 has the whole.
 __device__ __forceinline__ LpPart join_lanes(LpPart p, int count, float c) {
   for (int d = 1; d < count; d <<= 1) {
-    const LpPart o = {__shfl_xor_sync(kAll, p.m, d), __shfl_xor_sync(kAll, p.s, d), __shfl_xor_sync(kAll, p.a, d),
+    const LpPart o = {__shfl_xor_sync(kAll, p.s, d), __shfl_xor_sync(kAll, p.a, d),
                       __shfl_xor_sync(kAll, p.top_key, d)};
     p = join(p, o, c);
   }
@@ -172,12 +166,10 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
     return *reinterpret_cast<uint4*>(e);
   };
 
-  // the maximum and M are the warp's, S and A this lane's, in two halves (packed arithmetic)
+  // the maximum is the warp's, S and A this lane's, in two halves (packed arithmetic)
   const float ninf = -__int_as_float(0x7f800000);
   float most = ninf;
   bool bad = false;  // a NaN or +inf
-  float by = c;
-  float m = 0.0f;
   unsigned long long s2 = 0, a2 = 0;
   auto add = [&](int seg, const uint4 (&v)[kLpGroup]) {
     float rise = T::largest(v[0]);
@@ -188,15 +180,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
     if (rise == ninf) return;  // nothing but masked logits
     if (!(rise <= most)) {  // the same in all lanes
       if (rise < __int_as_float(0x7f800000)) {
-        const float last = by;
-        by = factor(rise, c);
-        const float next = rise * by;
         if (most != ninf) {
-          const float t = last == by ? fmaxf(m - next, -256.0f) : -256.0f, shrink = exp2f(t);
+          const float t = apart(most, rise, c), shrink = exp2f(t);
           a2 = f2_mul(f2_fma(s2, f2_pack(t, t), a2), f2_pack(shrink, shrink));
           s2 = f2_mul(s2, f2_pack(shrink, shrink));
         }
-        m = next;
         most = rise;
       } else {
         bad = true;
@@ -208,7 +196,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
       T::unpack(v[g], f);
 #pragma unroll
       for (int i = 0; i < kVec; i += 2) {
-        const float2 d = f2_unpack(f2_fma(f2_pack(f[i], f[i + 1]), f2_pack(by, by), f2_pack(-m, -m)));
+        const float2 d =
+            f2_unpack(f2_mul(f2_add(f2_pack(f[i], f[i + 1]), f2_pack(-most, -most)), f2_pack(c, c)));
         const float t0 = fmaxf(d.x, -256.0f), t1 = fmaxf(d.y, -256.0f);  // masked logits: 2^t = 0 and t finite
         const unsigned long long e = f2_pack(ex2_approx(t0), ex2_approx(t1));
         s2 = f2_add(s2, e);
@@ -267,7 +256,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
     add(seg + i * kLpWarps, v);
   }
   const float2 s_halves = f2_unpack(s2), a_halves = f2_unpack(a2);
-  LpPart p = {m, s_halves.x + s_halves.y, a_halves.x + a_halves.y, bad ? kAll : order_key(most)};
+  LpPart p = {s_halves.x + s_halves.y, a_halves.x + a_halves.y, bad ? kAll : order_key(most)};
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
     p.s += __shfl_xor_sync(kAll, p.s, d);
@@ -380,8 +369,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
     for (int r = 0; r < kLpMaxRanks; ++r)  // all remote reads in flight together
       lists_of[r] = a.top && r < ranks ? cluster.map_shared_rank(cta_list, r)[lane] : 0ull;
     LpPart all = join_lanes(*cluster.map_shared_rank(&cta_part, lane & (ranks - 1)), ranks, c);
-    all.m = __shfl_sync(kAll, all.m, 0);  // one lane's sums, so that a token has one value wherever it is listed
-    all.s = __shfl_sync(kAll, all.s, 0);
+    all.s = __shfl_sync(kAll, all.s, 0);  // one lane's sum, so that a token has one value wherever it is listed
 #pragma unroll
     for (int half = kLpMaxRanks / 2; half; half >>= 1)
       if (half < ranks) {
@@ -393,8 +381,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
     const bool bad = all.top_key >= 0xff800000u;  // +inf or NaN
     const bool empty = all.top_key == 0u;
     const float log_total = log2f(all.s);
-    // log p(m) = log 2 ((c m - M) - log2 S), of which c m - M is what M's rounding left
-    const float m = key_value(all.top_key), log_p_m = (fmaf(m, factor(m, c), -all.m) - log_total) * kLn2;
+    const float m = key_value(all.top_key), log_p_m = -log_total * kLn2;
     auto logp = [&](float x) { return bad ? nan : empty || x == ninf ? ninf : fmaf(x - m, a.scale, log_p_m); };
     if (lane == 0) {
       if (a.logprobs) a.logprobs[row] = has_given ? logp(given) : 0.0f;
