@@ -145,3 +145,14 @@ def test_logprobs_extreme_scales(device, dtype, scale):
     rows[4] = 33333.0
     logits = rows.to(DTYPES[dtype])
     check_logprobs(device, logits, torch.randint(3000, (6,), generator=g), 20, scale=scale)
+
+
+def test_logprobs_differences_beyond_the_largest_float(device):
+    """Logits further apart than FP32 holds, brought back into its range by the scale."""
+    rows = torch.full((3, 70), 3e38)
+    rows[0, 5:] = -3e38
+    rows[1, :69] = -2.5e38
+    rows[2, ::2] = -3.4e38
+    for scale in (1e-6, 0.1, 0.5):
+        check_logprobs(device, rows, torch.tensor([60, 3, 4]), 8, scale=scale)
+        check_logprobs(device, rows.bfloat16(), torch.tensor([60, 3, 4]), 8, scale=scale)

@@ -382,7 +382,10 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs(LpArgs a) {
     const bool empty = all.top_key == 0u;
     const float log_total = log2f(all.s);
     const float m = key_value(all.top_key), log_p_m = -log_total * kLn2;
-    auto logp = [&](float x) { return bad ? nan : empty || x == ninf ? ninf : fmaf(x - m, a.scale, log_p_m); };
+    // (over halves: the difference of two finite logits stays finite)
+    auto logp = [&](float x) {
+      return bad ? nan : empty || x == ninf ? ninf : fmaf(0.5f * x - 0.5f * m, 2.0f * a.scale, log_p_m);
+    };
     if (lane == 0) {
       if (a.logprobs) a.logprobs[row] = has_given ? logp(given) : 0.0f;
       if (a.entropy) a.entropy[row] = bad ? nan : empty ? 0.0f : (log_total - all.a / all.s) * kLn2;
