@@ -1,7 +1,7 @@
 // Gated products of the chosen experts:
 //   out[t] = sum_j w[t][j] down[e] (silu(gate[e] x[t]) * (up[e] x[t])),  e = experts[t][j].
 //
-// Few pairs (token, choice; few_pairs says how few): the experts' weights are read once for
+// Few pairs (token, choice; up to few_pairs): the experts' weights are read once for
 // each pair by ordinary warps, two launches in all (expert_rows_gate_up, expert_rows_down).
 //
 // More pairs: the tensor cores, three or four launches.
@@ -25,6 +25,7 @@
 //  * expert_combine adds a token's shares in the order of its choices.
 // Every wait is bounded (200 ms); a role that gives up records why in a device word
 // (ttn_expert_mlp_fault) and the pair frees its TMEM and returns.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -703,16 +704,16 @@ __global__ void __launch_bounds__(kCombineThreads, 3) expert_combine(ExpertArgs 
   *reinterpret_cast<uint2*>(a.out + token * a.out_stride + f) = make_uint2(T::round2(sum[0], sum[1]), T::round2(sum[2], sum[3]));
 }
 
-// Whether each pair reads its expert's weights by itself, on ordinary warps: where all those
-// readings are few bytes, or few pairs meet many experts, so that they read most of them once.
+// Up to how many pairs each reads its expert's weights by itself, on ordinary warps: where all
+// those readings are few bytes, or few pairs meet many experts, so that they read most of them once.
 // The tensor cores' four dependent launches take 15 us and more.  Both sides measured (rows /
 // tensor cores, us; bf16): hidden 256, inner 128, 8 experts: 128 pairs 8.7 / 15.1, 256 pairs 14.5 /
 // 15.6, 512 pairs 26 / 17; 512, 256, 16: 128 pairs (101 MB) 16.1 / 16.8; 1024, 512, 32: 40 pairs
 // (126 MB) 24 / 32, 64 pairs 32 / 33, 128 pairs 51 / 33; 2048, 1024, 8: 20 pairs (252 MB) 34 / 29;
 // 2048, 1024, 64: 32 pairs (403 MB) 63 / 73, 48 pairs 87 / 80.
-bool few_pairs(int64_t pairs, int64_t hidden, int64_t inner, int64_t experts) {
+int64_t few_pairs(int64_t hidden, int64_t inner, int64_t experts) {
   const int64_t bytes = 6 * hidden * inner;  // of one expert's weights
-  return (pairs <= 256 && pairs * bytes <= 128 * 1000 * 1000) || (pairs <= 32 && 2 * pairs <= experts);
+  return std::max(std::min<int64_t>(256, 128 * 1000 * 1000 / bytes), std::min<int64_t>(32, experts / 2));
 }
 
 // Whether the first product takes two sub-tiles: experts with many rows, no more padding of
@@ -738,7 +739,8 @@ bool sizes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64
     return false;
   auto pad = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
   s->pairs = tokens * top_k;
-  s->rows = few_pairs(s->pairs, hidden, inner, experts);
+  const int64_t few = few_pairs(hidden, inner, experts);
+  s->rows = s->pairs <= few;
   if (s->rows) {
     s->order = s->h = s->share = 0;
     s->total = pad(s->pairs * inner * 4);
@@ -746,7 +748,8 @@ bool sizes(int64_t tokens, int64_t hidden, int64_t inner, int64_t experts, int64
     s->order = pad((experts + 1) * 4);
     s->h = s->order + pad(s->pairs * 4);
     s->share = s->h + pad(s->pairs * inner * 2);
-    s->total = s->share + pad(s->pairs * hidden * 4);
+    // never less than a smaller batch needs, whose activations are FP32
+    s->total = std::max(s->share + pad(s->pairs * hidden * 4), pad(few * inner * 4));
   }
   return true;
 }

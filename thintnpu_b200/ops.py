@@ -715,7 +715,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
 
 
 def expert_mlp_workspace_size(tokens: int, hidden: int, inner: int, num_experts: int, top_k: int) -> int:
-    """Bytes of scratch ``expert_mlp`` needs at these sizes."""
+    """Bytes of scratch ``expert_mlp`` needs at these sizes: enough for fewer tokens too."""
     return int(_lib.lib().ttn_expert_mlp_workspace_size(tokens, hidden, inner, num_experts, top_k))
 
 
