@@ -449,9 +449,9 @@ ttn_status ttn_token_logprobs(const ttn_tensor* logits, const int64_t* tokens, f
  * gets zeros.  Products accumulate in FP32; the gated activations are rounded to dtype
  * between the two products where the tensor cores take them (so they have to lie in its
  * range), with few pairs not.  hidden % 8 == 0, inner % 16 == 0 (both up to 2^20),
- * num_experts 1..1024, top_k 1..32, tokens * top_k <= (2^31 - 1) / 256; 16-byte aligned
- * bases, row strides multiples of 8 and at least hidden.  workspace: at least
- * ttn_expert_mlp_workspace_size bytes (0 for malformed sizes), 256-byte aligned, used by
+ * num_experts 1..1024, top_k 1..32, tokens * top_k <= (2^31 - 1) / 256, tokens * hidden
+ * <= 2^34 - 4096; 16-byte aligned bases, row strides multiples of 8 and at least hidden.
+ * workspace: at least ttn_expert_mlp_workspace_size bytes (0 for malformed sizes), 256-byte aligned, used by
  * one call at a time; the size never falls as tokens rise. */
 size_t ttn_expert_mlp_workspace_size(int64_t tokens, int64_t hidden, int64_t inner, int64_t num_experts,
                                      int64_t top_k);

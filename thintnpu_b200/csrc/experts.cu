@@ -816,7 +816,6 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     p.m_tiles = (rows + tile - 1) / tile;
     p.bf16 = bf16;
     p.withhold = gate_up && g_withhold_next_products.exchange(false);
-    if (runs * p.m_tiles > INT32_MAX) return fail(TTN_UNSUPPORTED, "%s: more than 2^31 tiles", name);
     TTN_TRY(ensure_dynamic_smem((const void*)kernel, (int)smem));
     const int64_t pairs_of_sms = sm_count() / 2, most = runs * p.m_tiles;
     const unsigned grid = 2 * (unsigned)(most < pairs_of_sms ? most : pairs_of_sms);
@@ -828,7 +827,6 @@ ttn_status launch_products(const char* name, const ExpertArgs& a, const Sizes& s
     TTN_TRY(products(expert_products<T, true, 1>, true, 1, gate, a.inner, a.hidden));
   TTN_TRY(products(expert_products<T, false, 1>, false, 1, down, a.hidden, a.inner));
   const int64_t items = a.tokens * (a.hidden / 4);
-  if (items + kCombineThreads > UINT32_MAX) return fail(TTN_UNSUPPORTED, "%s: output too large", name);
   return cuda_check(launch_pdl(expert_combine<T>, dim3((unsigned)((items + kCombineThreads - 1) / kCombineThreads)),
                                dim3(kCombineThreads), 0, stream, a, (const float*)share,
                                FastDiv((uint32_t)(a.hidden / 4))),
@@ -841,8 +839,6 @@ ttn_status launch_experts(const char* name, const ExpertArgs& a, const Sizes& s,
   float* h = (float*)workspace;
   const int64_t pairs = s.pairs;
   const int gate_blocks = (a.inner + kRowsBlock - 1) / kRowsBlock, down_blocks = a.hidden / kDownRows;
-  if (pairs * gate_blocks > INT32_MAX || a.tokens * down_blocks > INT32_MAX)
-    return fail(TTN_UNSUPPORTED, "%s: too many tokens for these sizes", name);
   expert_rows_gate_up<T><<<(unsigned)(pairs * gate_blocks), kRowsThreads, 0, stream>>>(a, h, gate_blocks);
   TTN_TRY(launch_check(name));
   const int warps = a.top_k < kDownWarps ? a.top_k : kDownWarps;
@@ -879,6 +875,9 @@ ttn_status ttn_expert_mlp(int dtype, const void* x, int64_t x_row_stride, int64_
                 (long long)top_k, kMaxChoices);
   if (hidden % 8 || inner % 16)
     return fail(TTN_UNSUPPORTED, "%s: hidden must be a multiple of 8 and inner of 16", name);
+  // the combine's 32-bit index of 4 outputs; 2^23 pairs and 2^20 rows keep every other count below 2^31
+  if (tokens * hidden > (1ll << 34) - 4096)
+    return fail(TTN_UNSUPPORTED, "%s: tokens * hidden must be below 2^34 - 4095", name);
   if (tokens == 0) return TTN_OK;
   if (!x || !experts || !weights || !gate_up || !down || !out) return fail(TTN_INVALID_ARG, "%s: null pointer", name);
   if (((uintptr_t)x | (uintptr_t)gate_up | (uintptr_t)down | (uintptr_t)out) % 16)
