@@ -48,6 +48,22 @@ def test_mlp_shares_near_the_largest_float(device, tokens, peak):
     check_mlp(got, args)
 
 
+def test_mlp_calls_of_few_and_many_tiles_in_turn(device):
+    """Calls with fewer ring steps than stages, with one tile and with several a CTA pair, close
+    behind one another: each is right, repeats itself and leaves no wait unfinished."""
+    import thintnpu_b200 as ttn
+    sets = [mlp_inputs(tokens, hidden, inner, experts, 1, torch.bfloat16, tokens)
+            for tokens, hidden, inner, experts in ((300, 64, 16, 1), (2600, 72, 1024, 2), (270, 520, 48, 9), (9000, 64, 1024, 3))]
+    dev = [[t.to(device) for t in args] for args in sets]
+    first = [ttn.expert_mlp(*args) for args in dev]
+    for _ in range(20):
+        again = [ttn.expert_mlp(*args) for args in dev]
+    assert ttn.ops.expert_mlp_fault() == 0
+    for args, a, b in zip(sets, first, again):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+        check_mlp(a, args)
+
+
 # ------------------------------------------------------------------ route_experts
 
 @pytest.mark.parametrize("size", [3, 4])

@@ -479,6 +479,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(kGat
         if (++s == kStages) s = 0, phase ^= 1;
       }
     }
+    // The leader's commits arrive in this CTA too: none may be on its way when the CTA exits.
+    for (int i = 0; i < kStages && !fault && !a.withhold; ++i) {
+      if (!__all_sync(kAll, mbar_wait_cluster(empty_bar(s), phase ^ 1))) fault = 2;
+      if (++s == kStages) s = 0, phase ^= 1;
+    }
   } else if (kGateUp && warp >= 2 + kEpiWarps) {
     // Gathering warps, one thread each: every fourth copy of four rows.  A stage has 16 rows at
     // least, so each warp has a part in every stage: none falls two phases of a barrier
