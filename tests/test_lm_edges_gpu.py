@@ -172,3 +172,39 @@ def test_logprobs_differences_beyond_the_largest_float(device):
     for scale in (1e-6, 0.1, 0.5):
         check_logprobs(device, rows, torch.tensor([60, 3, 4]), 8, scale=scale)
         check_logprobs(device, rows.bfloat16(), torch.tensor([60, 3, 4]), 8, scale=scale)
+
+
+# ------------------------------------------------------------------ alone and in a batch
+
+def test_a_row_alone_agrees_with_the_row_in_a_batch(device):
+    """The number of rows decides the kernels of expert_mlp and the CTAs a row of
+    token_logprobs, and a row's address where its vectors begin: values agree within twice the
+    bounds that each is held to, the router's bitwise."""
+    import thintnpu_b200 as ttn
+    g = torch.Generator().manual_seed(23)
+    logits = torch.randn(500, 60, generator=g)
+    weights, ids = ttn.route_experts(logits.to(device), 4, score="sigmoid", renormalize=True)
+    for row in (0, 7, 499):
+        w, i = ttn.route_experts(logits[row:row + 1].to(device), 4, score="sigmoid", renormalize=True)
+        assert torch.equal(w, weights[row:row + 1]) and torch.equal(i, ids[row:row + 1])
+
+    args = mlp_inputs(300, 200, 96, 5, 2, torch.bfloat16, 29)
+    want, err = lm.expert_mlp(*args)
+    half = torch.finfo(torch.bfloat16).eps / 2
+    bound = 2 * (err + half * (want.abs() + err) + torch.finfo(torch.bfloat16).smallest_normal * half)
+    dev = [t.to(device) for t in args]
+    batch = ttn.expert_mlp(*dev).cpu().double()
+    for rows in (1, 40):
+        part = ttn.expert_mlp(*(t[:rows] for t in dev[:3]), *dev[3:]).cpu().double()
+        assert bool(((part - batch[:rows]).abs() <= bound[:rows]).all())
+
+    scores = (torch.randn(321, 20011, generator=g) * 3).to(device)  # odd rows: every alignment
+    tokens = torch.randint(20011, (321,), generator=g).to(device)
+    batch = [t.cpu().double() for t in ttn.token_logprobs(scores, tokens, top=4)]
+    for row in (0, 1, 2, 320):
+        alone = [t.cpu().double() for t in ttn.token_logprobs(scores[row:row + 1].clone(), tokens[row:row + 1], top=4)]
+        assert torch.equal(alone[3], batch[3][row:row + 1])
+        for n, (a, b) in enumerate(zip(alone[:3], batch[:3])):
+            b = b[row:row + 1]
+            z = torch.full_like(b, (math.log(20011) + 1) * (20011 / 256 + 64) / 8) if n == 1 else b.abs() + math.log(20012)
+            assert bool(((a - b).abs() <= 2 * (8 * z + 20011 / 256 + 64) * 2.0 ** -24).all())
