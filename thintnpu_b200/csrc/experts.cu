@@ -180,7 +180,8 @@ std::atomic<bool> g_withhold_next_products{false};
 
 // offsets[e]: pairs of experts below e; order: the pairs, by expert, then by number.  One
 // block an expert, each reading all ids twice (they are few and in L2), 128 a warp and load:
-// no block waits for another.  65,536 ids of 64 experts take 8 us on a B200.
+// no block waits for another.  The reading grows with experts x pairs: on a B200 65,536 ids of 64
+// experts take 12 us and of 256 experts 19 us, 32,768 ids of 1024 experts 27 us.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kPlanBatch = 4;  // loads in flight
