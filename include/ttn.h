@@ -406,9 +406,9 @@ ttn_status ttn_select_f16_static(const ttn_tensor* decoded, int64_t max_det, uin
  * ranks each by its best rank (group_top 1) or the sum of its two best (2) and keeps
  * the top_groups best.  The top_k (1..16) experts by rank are chosen from those;
  * experts [rows, top_k] int32 receives them in falling rank, equal ranks (of experts
- * and of groups) in index order, and weights [rows, top_k] f32 their s (without the bias) times `scale`,
- * with TTN_ROUTE_RENORMALIZE divided by the sum of the chosen s first (0 where that is
- * 0).  The order is that of the exact ranks: fp32 scores too close to tell apart are
+ * and of groups) in index order, and weights [rows, top_k] f32 their s (without the bias)
+ * times `scale`, with TTN_ROUTE_RENORMALIZE divided by the sum of the chosen s first (0 where
+ * that is 0 in 64 bits, as for logits of the lowest value under a sigmoid).  The order is that of the exact ranks: fp32 scores too close to tell apart are
  * ranked again in 64 bits, and without a bias the logits themselves are compared.
  * A logit of -inf masks its expert, and so does a bias of -inf (which leaves it in a
  * softmax row's total): it is never chosen, and choices for which no expert is left get

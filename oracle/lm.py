@@ -52,6 +52,10 @@ def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, 
             s = {e: math.nan if math.isnan(v[e]) else 1 / (1 + math.exp(-v[e])) if v[e] > -700 else math.exp(v[e])
                  for e in open_}
         rank = {e: s[e] + (0.0 if bias is None else float(bias[e])) for e in open_}
+        if bias is None and (groups == 1 or group_top == 1 or experts == groups):
+            # both scores rise with the logit, so its order is the exact one where 64 bits hold the
+            # scores no more (0 below -745, 1 above 37)
+            rank = {e: rank[e] if math.isnan(rank[e]) else v[e] for e in open_}
         open_ = [e for e in open_ if rank[e] != -math.inf]  # a bias of -inf masks an expert as a logit does
         rank = {e: rank[e] for e in open_}
         if groups > 1:

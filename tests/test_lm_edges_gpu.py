@@ -128,6 +128,34 @@ def test_route_group_sums_beyond_the_largest_float(device, experts):
     check_route(device, logits, 3, score="sigmoid", bias=bias, groups=groups, top_groups=1, group_top=2)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_route_renormalised_scores_that_all_vanish(device, dtype, groups):
+    """Rows under a finite mask of the type's lowest value, or with all chosen logits far below:
+    their scores are 0 in 64 bits, and so are the weights (not equal shares)."""
+    low = torch.finfo(DTYPES[dtype]).min
+    g = torch.Generator().manual_seed(8)
+    logits = torch.randn(7, 16, generator=g)
+    logits[0] = low
+    logits[1, 1:] = low                 # one ordinary expert
+    logits[2] = -1000.0 + logits[3]
+    logits[4] = -600.0                  # small, but not 0 in 64 bits
+    logits[5, 3:] = low
+    logits[6] = -math.inf
+    logits[6, 5:9] = low
+    logits = logits.to(DTYPES[dtype])
+    for top_k in (1, 4, 7):
+        check_route(device, logits, top_k, score="sigmoid", groups=groups, top_groups=max(1, groups // 2), renormalize=True)
+    # a softmax whose chosen experts, wanted by their biases, are far below the row's largest
+    logits = torch.randn(4, 16, generator=g)
+    logits[:, 4:] -= 60000.0
+    logits[1:, 4:] = low
+    bias = torch.zeros(16)
+    bias[8:] = 2.0
+    check_route(device, logits.to(DTYPES[dtype]), 4, score="softmax", bias=bias, groups=groups,
+                top_groups=max(1, groups // 2), renormalize=True)
+
+
 # ------------------------------------------------------------------ token_logprobs
 
 @pytest.mark.parametrize("vocabulary,top", [(40, 8), (5000, 20)])

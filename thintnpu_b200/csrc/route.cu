@@ -455,10 +455,12 @@ __global__ void __launch_bounds__(kRouteThreads, W <= 8 ? 12 : 4) route_rows(Rou
 
   // Weights, one choice a lane.  Renormalised softmax needs only the chosen logits, taken
   // relative to their own maximum; so do sigmoids so small that s = e^x to fp32 (x < -20).
+  // Where all chosen scores are 0 in 64 bits (logits of the lowest value), so is their sum.
   const float xm = mine >= 0 ? logit<T>(a, row, mine) : ninf;
   float s = 0.0f;
   const float chosen = a.renormalize ? warp_largest(xm) : 0.0f;
-  if (mine >= 0) {
+  const bool vanished = a.renormalize && (a.sigmoid ? chosen : chosen - m) < -745.13322f;  // e^that < 2^-1074
+  if (mine >= 0 && !vanished) {
     if (a.sigmoid)
       s = a.renormalize && chosen < -20.0f ? expf(xm - chosen) : __fdividef(1.0f, 1.0f + expf(-xm));
     else
