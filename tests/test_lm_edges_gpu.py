@@ -236,3 +236,41 @@ def test_a_row_alone_agrees_with_the_row_in_a_batch(device):
             b = b[row:row + 1]
             z = torch.full_like(b, (math.log(20011) + 1) * (20011 / 256 + 64) / 8) if n == 1 else b.abs() + math.log(20012)
             assert bool(((a - b).abs() <= 2 * (8 * z + 20011 / 256 + 64) * 2.0 ** -24).all())
+
+
+# ------------------------------------------------------------------ far offsets
+
+def test_offsets_beyond_32_bits(device):
+    """Rows 2^31 elements apart, and experts whose weights begin beyond 2^31 elements."""
+    import thintnpu_b200 as ttn
+    g = torch.Generator().manual_seed(31)
+    far = 2 ** 31 + 64
+    buffer = torch.zeros(far + 2048, dtype=torch.bfloat16, device=device)
+
+    def spread(rows):  # two rows, far apart
+        view = buffer.as_strided((2, rows.size(1)), (far, 1))
+        view.copy_(rows)
+        return view
+
+    logits = torch.randn(2, 96, generator=g).bfloat16()
+    check_route(device, logits, 5, dev_logits=spread(logits), score="sigmoid", renormalize=True)
+    scores = torch.randn(2, 1500, generator=g).bfloat16()
+    check_logprobs(device, scores, torch.tensor([3, 1499]), 7, dev_logits=spread(scores))
+
+    experts, hidden, inner = 1000, 2048, 544
+    used = [0, 510, 998, 999]  # gate_up of the last two begins beyond 2^31 elements
+    x, ids, weights, gate_up, down = mlp_inputs(200, hidden, inner, len(used), 2, torch.bfloat16, 37)
+    all_gate_up = torch.empty(experts, 2 * inner, hidden, dtype=torch.bfloat16, device=device)
+    all_down = torch.empty(experts, hidden, inner, dtype=torch.bfloat16, device=device)
+    all_gate_up[used] = gate_up.to(device)
+    all_down[used] = down.to(device)
+    all_ids = torch.tensor(used, dtype=torch.int32)[ids.long()].to(device)
+    for rows in (2, 200):
+        got = ttn.expert_mlp(x[:rows].to(device), all_ids[:rows], weights[:rows].to(device), all_gate_up, all_down)
+        check_mlp(got, (x[:rows], ids[:rows], weights[:rows], gate_up, down))
+    # two tokens far apart, in and out, on the tensor cores: more pairs than the other kernels take
+    ids, weights = torch.randint(0, 4, (2, 32), generator=g, dtype=torch.int32), torch.rand(2, 32, generator=g)
+    out = torch.zeros(far + 2048, dtype=torch.bfloat16, device=device).as_strided((2, hidden), (far, 1))
+    got = ttn.expert_mlp(spread(x[:2]), torch.tensor(used, dtype=torch.int32)[ids.long()].to(device), weights.to(device),
+                         all_gate_up, all_down, out=out)
+    check_mlp(got, (x[:2], ids, weights, gate_up, down))
