@@ -156,6 +156,15 @@ def test_route_renormalised_scores_that_all_vanish(device, dtype, groups):
                 top_groups=max(1, groups // 2), renormalize=True)
 
 
+def test_route_refuses_whole_numbers_that_would_wrap(device):
+    import thintnpu_b200 as ttn
+    logits = torch.randn(3, 16, device=device)
+    for kw, message in ((dict(group_top=2 ** 32 + 1), "group_top"), (dict(groups=2 ** 64 + 4, top_groups=2), "groups"),
+                        (dict(groups=4, top_groups=2 ** 64 + 1), "top_groups"), (dict(groups=-4), "groups")):
+        with pytest.raises(RuntimeError, match=message):
+            ttn.route_experts(logits, 2, **kw)
+
+
 # ------------------------------------------------------------------ token_logprobs
 
 @pytest.mark.parametrize("vocabulary,top", [(40, 8), (5000, 20)])

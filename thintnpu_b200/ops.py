@@ -700,6 +700,13 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     top_k = int(top_k)
     if not 1 <= top_k <= experts:
         _fail(f"{what}: top_k must be in [1, experts]")
+    top_groups = groups if top_groups is None else top_groups
+    if not 1 <= groups <= 32:  # (ctypes would take these modulo 2^64 and 2^32)
+        _fail(f"{what}: groups must divide the experts and be in [1, 32]")
+    if not 1 <= top_groups <= groups:
+        _fail(f"{what}: top_groups must be in [1, groups]")
+    if group_top not in (1, 2):
+        _fail(f"{what}: group_top must be 1 or 2")
     if out is None:
         weights = logits.new_empty((rows, top_k), dtype=torch.float32)
         ids = logits.new_empty((rows, top_k), dtype=torch.int32)
@@ -708,9 +715,8 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
         _like_output(weights, (rows, top_k), torch.float32, device, "route_experts: out weights")
         _like_output(ids, (rows, top_k), torch.int32, device, "route_experts: out experts")
     flags = (_lib.ROUTE_SIGMOID if score == "sigmoid" else 0) | (_lib.ROUTE_RENORMALIZE if renormalize else 0)
-    _call_on(device, "ttn_route_experts", _rows(logits, dtype), bias_ptr, top_k, groups,
-             groups if top_groups is None else top_groups, group_top, flags, scale, weights.data_ptr(),
-             ids.data_ptr())
+    _call_on(device, "ttn_route_experts", _rows(logits, dtype), bias_ptr, top_k, groups, top_groups, group_top, flags,
+             scale, weights.data_ptr(), ids.data_ptr())
     return weights, ids
 
 
