@@ -406,14 +406,16 @@ ttn_status ttn_select_f16_static(const ttn_tensor* decoded, int64_t max_det, uin
  * ranks each by its best rank (group_top 1) or the sum of its two best (2) and keeps
  * the top_groups best.  The top_k (1..16) experts by rank are chosen from those;
  * experts [rows, top_k] int32 receives them in falling rank, equal ranks (of experts
- * and of groups) in index order, and weights [rows, top_k] f32 their s (without the bias)
- * times `scale`, with TTN_ROUTE_RENORMALIZE divided by the sum of the chosen s first (0 where
- * that is 0 in 64 bits, as for logits of the lowest value under a sigmoid).  The order is that of the exact ranks: fp32 scores too close to tell apart are
- * ranked again in 64 bits, and without a bias the logits themselves are compared.
- * A logit of -inf masks its expert, and so does a bias of -inf (which leaves it in a
- * softmax row's total): it is never chosen, and choices for which no expert is left get
- * id -1 and weight 0.  A bias of +inf ranks its expert before all finite ones.  A NaN ranks first; in a softmax row a NaN or
- * +inf makes every score NaN.  Both outputs contiguous. */
+ * and of groups) in index order, and weights [rows, top_k] f32 their s (without the
+ * bias) times `scale`, with TTN_ROUTE_RENORMALIZE divided by the sum of the chosen s
+ * first (0 where that is 0 in 64 bits, as for logits of the lowest value under a
+ * sigmoid); a score below 2^-126 that is not renormalised may count as 0.  The order is
+ * that of the exact ranks: fp32 scores too close to tell apart are ranked again in 64
+ * bits, and without a bias the logits themselves are compared. A logit of -inf masks
+ * its expert, and so does a bias of -inf (which leaves it in a softmax row's total): it
+ * is never chosen, and choices for which no expert is left get id -1 and weight 0.  A
+ * bias of +inf ranks its expert before all finite ones.  A NaN ranks first; in a
+ * softmax row a NaN or +inf makes every score NaN.  Both outputs contiguous. */
 #define TTN_ROUTE_SIGMOID 1u
 #define TTN_ROUTE_RENORMALIZE 2u
 ttn_status ttn_route_experts(const ttn_tensor* logits, const float* bias, int64_t top_k, int64_t groups,
@@ -448,11 +450,12 @@ ttn_status ttn_token_logprobs(const ttn_tensor* logits, const int64_t* tokens, f
  * (-1: no choice; another rank's experts) add nothing; a token without any other id
  * gets zeros.  Products accumulate in FP32; the gated activations are rounded to dtype
  * between the two products where the tensor cores take them (so they have to lie in its
- * range), with few pairs not.  hidden % 8 == 0, inner % 16 == 0 (both up to 2^20),
- * num_experts 1..1024, top_k 1..32, tokens * top_k <= (2^31 - 1) / 256, tokens * hidden
- * <= 2^34 - 4096; 16-byte aligned bases, row strides multiples of 8 and at least hidden.
- * workspace: at least ttn_expert_mlp_workspace_size bytes (0 for malformed sizes), 256-byte aligned, used by
- * one call at a time; the size never falls as tokens rise. */
+ * range), with few pairs not; silu(v) for v < -87, below 2^-119, counts as 0.  hidden %
+ * 8 == 0, inner % 16 == 0 (both up to 2^20), num_experts 1..1024, top_k 1..32, tokens *
+ * top_k <= (2^31 - 1) / 256, tokens * hidden <= 2^34 - 4096; 16-byte aligned bases, row
+ * strides multiples of 8 and at least hidden. workspace: at least
+ * ttn_expert_mlp_workspace_size bytes (0 for malformed sizes), 256-byte aligned, used
+ * by one call at a time; the size never falls as tokens rise. */
 size_t ttn_expert_mlp_workspace_size(int64_t tokens, int64_t hidden, int64_t inner, int64_t num_experts,
                                      int64_t top_k);
 ttn_status ttn_expert_mlp(int dtype, const void* x, int64_t x_row_stride, int64_t tokens, int64_t hidden,
@@ -462,7 +465,8 @@ ttn_status ttn_expert_mlp(int dtype, const void* x, int64_t x_row_stride, int64_
 
 /* Reads and clears the fault word of the experts' products: nonzero when a launch gave
  * up waiting (1 = an operand copy, 2 = a free ring stage, 4 = an accumulator); its
- * output is then incomplete.  Synchronous. */
+ * output is then incomplete.  It speaks of launches on the current device that have
+ * finished: wait for their streams first.  Synchronous. */
 ttn_status ttn_expert_mlp_fault(uint32_t* fault);
 
 /* Test hook for the bounded waits above: the next ttn_expert_mlp call that takes the

@@ -737,8 +737,9 @@ def expert_mlp(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, ga
     contiguous, of x's dtype; hidden a multiple of 8, inner of 16.  Ids outside 0..E-1
     add nothing (-1: no choice; experts of another rank).  Sums are FP32; the gated
     activations are rounded to x's dtype between the two products (with few pairs they
-    stay FP32), so they have to lie in its range.  ``workspace``: at least
-    ``expert_mlp_workspace_size`` bytes of uint8, 256-byte aligned, for one call at a time."""
+    stay FP32), so they have to lie in its range.  ``out`` must not overlap the inputs.
+    ``workspace``: at least ``expert_mlp_workspace_size`` bytes of uint8, 256-byte aligned,
+    for one call at a time."""
     what = "expert_mlp"
     _inputs(what, x, experts, weights, gate_up, down)
     device, dtype = x.device, x.dtype
@@ -775,7 +776,8 @@ def expert_mlp(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, ga
 
 
 def expert_mlp_fault() -> int:
-    """Reads and clears the experts' products' fault word (0 = no launch gave up)."""
+    """Reads and clears the experts' products' fault word of the current device: 0 where no
+    launch that has finished gave up (wait for its stream first)."""
     word = ctypes.c_uint32(0)
     call("ttn_expert_mlp_fault", ctypes.byref(word))
     return int(word.value)
